@@ -29,7 +29,11 @@ ext = CUDAExtension(
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
-        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+        # no packed fp32 instructions: some of their forms have given
+        # wrong results on this card now and then, without an error
+        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
+                 "-Xclang", "-target-feature",
+                 "-Xclang", "-packed-fp32-ops"],
     },
 )
 

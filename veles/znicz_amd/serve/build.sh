@@ -9,7 +9,7 @@ SRCS="mzserve.cpp ../ops/hip/gemm.hip ../ops/hip/gemm8.hip \
       ../ops/hip/elementwise.hip ../ops/hip/softmax.hip \
       ../ops/hip/pool_lrn.hip"
 DEPS="$SRCS ../ops/hip/api.h ../ops/hip/common.h ../ops/hip/loaders.h \
-      ../ops/hip/sgd_multi.h"
+      ../ops/hip/sgd_multi.h build.sh"
 if [ -x mzserve ]; then
   stale=0
   for f in $DEPS; do
@@ -17,5 +17,8 @@ if [ -x mzserve ]; then
   done
   [ "$stale" = 0 ] && { echo "mzserve up to date"; exit 0; }
 fi
-hipcc -O3 -std=c++17 --offload-arch=gfx950 -x hip $SRCS -o mzserve
+# (no packed fp32 instructions: see ../ops/setup.py)
+hipcc -O3 -std=c++17 --offload-arch=gfx950 \
+      -Xclang -target-feature -Xclang -packed-fp32-ops \
+      -x hip $SRCS -o mzserve
 echo "built mzserve"
