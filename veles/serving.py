@@ -43,6 +43,8 @@ class InferenceEngine(object):
         wf.loader.initialize(device=device)
         for f in self.forwards:
             f.forward_mode = True      # inference: dropout = identity
+            if hasattr(f, "logits_only"):
+                f.logits_only = False  # (a distilled head is a softmax)
             f.initialize(device=device)
         self.batch_size = batch_size or int(wf.loader.max_minibatch_size)
         self._in = wf.loader.minibatch_data

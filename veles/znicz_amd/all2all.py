@@ -126,6 +126,10 @@ class All2AllSoftmax(All2All):
     MAPPING = "softmax"
     ACTIVATION = act.ACT_LINEAR
 
+    #: leave the logits in ``output`` (no softmax, no ``max_idx``): set by
+    #: who asks for log probabilities instead of probabilities
+    logits_only = False
+
     def __init__(self, workflow, **kwargs):
         super(All2AllSoftmax, self).__init__(workflow, **kwargs)
         self.max_idx = Array()
@@ -144,6 +148,8 @@ class All2AllSoftmax(All2All):
 
     def numpy_run(self):
         super(All2AllSoftmax, self).numpy_run()
+        if self.logits_only:
+            return
         v = self.output.mem
         self.max_idx.map_invalidate()
         self.max_idx.mem[...] = numpy.argmax(v, axis=1)
@@ -156,6 +162,8 @@ class All2AllSoftmax(All2All):
         x = ops.as2d_bf16(self.input)
         ops.gemm_nt(x, self._w_for_forward(), self.output.devmem,
                     bias=self.bias.devmem if self.include_bias else None)
-        ops.softmax_fwd(self.output.devmem, self.max_idx.devmem)
         self.output.touch_device()
+        if self.logits_only:
+            return
+        ops.softmax_fwd(self.output.devmem, self.max_idx.devmem)
         self.max_idx.touch_device()

@@ -139,29 +139,6 @@ class GradientDescentConv(GradientDescentBase):
             self.gradient_bias.touch_device()
         self._hip_apply(batch)
 
-    def _hip_apply(self, batch):
-        from veles.znicz_amd import ops
-        if not self.apply_gradient:
-            return
-        reducer = getattr(self.workflow, "grad_reducer", None)
-        if reducer is not None:
-            reducer.submit(self, batch)
-            return
-        scale = 1.0 / batch
-        ops.sgd_step(self.weights, self.gradient_weights.devmem,
-                     self.accumulated_gradient_weights.devmem,
-                     self.learning_rate, self.weights_decay, self.l1_vs_l2,
-                     self.gradient_moment, scale)
-        self.weights.touch_device()
-        if self.include_bias and self.bias is not None and self.bias:
-            ops.sgd_step(self.bias, self.gradient_bias.devmem,
-                         self.accumulated_gradient_bias.devmem,
-                         self.learning_rate_bias, self.weights_decay_bias,
-                         self.l1_vs_l2_bias, self.gradient_moment_bias,
-                         scale)
-            self.bias.touch_device()
-        self.post_update()
-
     def post_update(self):
         from veles.znicz_amd import ops
         ops.refresh_conv_copies(self.weights)

@@ -49,6 +49,8 @@ class GraphStepper(object):
         self.wf = workflow
         self.loader = workflow.loader
         self.forwards = list(workflow.forwards)
+        #: what runs between the forwards and the evaluator
+        self.teacher = getattr(workflow, "teacher", None)
         self.evaluator = workflow.evaluator
         self.decision = workflow.decision
         self.gds_rev = [g for g in reversed(workflow.gds)]
@@ -104,6 +106,8 @@ class GraphStepper(object):
             self.loader.device_gather_if_pending()
         for f in self.forwards:
             f.run()
+        if self.teacher is not None:
+            self.teacher.run()
         self.evaluator.run()
         for g in self.gds_rev:
             g.run()
@@ -114,6 +118,8 @@ class GraphStepper(object):
             self.loader.device_gather_if_pending()
         for f in self.forwards:
             f.run()
+        if self.teacher is not None:
+            self.teacher.run()
         self.evaluator.run()
         if check_skip:
             self.decision.run()

@@ -174,6 +174,30 @@ class GradientDescentBase(NNLayerBase):
         """Refresh derived weight images after an SGD apply (overridden
         by units that keep transposed/permuted bf16 copies)."""
 
+    def _hip_apply(self, batch):
+        """Apply SGD now, or hand the bucket to the DP reducer which will
+        apply it after the all-reduce completes (overlapped path)."""
+        from veles.znicz_amd import ops
+        if not self.apply_gradient:
+            return
+        reducer = getattr(self.workflow, "grad_reducer", None)
+        if reducer is not None:
+            reducer.submit(self, batch)
+            return
+        ops.sgd_step(self.weights, self.gradient_weights.devmem,
+                     self.accumulated_gradient_weights.devmem,
+                     self.learning_rate, self.weights_decay, self.l1_vs_l2,
+                     self.gradient_moment, 1.0 / batch)
+        self.weights.touch_device()
+        if self.include_bias and self.bias is not None and self.bias:
+            ops.sgd_step(self.bias, self.gradient_bias.devmem,
+                         self.accumulated_gradient_bias.devmem,
+                         self.learning_rate_bias, self.weights_decay_bias,
+                         self.l1_vs_l2_bias, self.gradient_moment_bias,
+                         1.0 / batch)
+            self.bias.touch_device()
+        self.post_update()
+
     # -- numpy reference update --------------------------------------------
     def numpy_apply_gradient(self, w_arr, g, acc_arr, lr, decay, l1_vs_l2,
                              moment):
@@ -234,6 +258,7 @@ class NNWorkflow(AcceleratedWorkflow):
         self.repeater = Repeater(self)
         self.loader = None
         self.forwards = []
+        self.teacher = None         # (distillation alone)
         self.evaluator = None
         self.decision = None
         self.gds = []

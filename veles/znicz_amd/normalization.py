@@ -128,3 +128,154 @@ class LRNormalizerBackward(GradientDescentBase):
                     None, self.err_input.devmem,
                     self.alpha, self.beta, self.k, self.n)
         self.err_input.touch_device()
+
+
+class LayerNormForward(Forward):
+    """Normalization over the last dimension (a sample's features, or the
+    channels at each place of a map) by its own mean and deviation:
+
+        y = (x − mean) / sqrt(var + eps) · weights + bias
+
+    ``weights`` (the gain, 1 at the start) and ``bias`` have one value for
+    each feature.  In training the row statistics are kept for the backward
+    unit; in ``forward_mode`` they are not written.  No reference
+    counterpart."""
+
+    MAPPING = "layer_norm"
+
+    def __init__(self, workflow, **kwargs):
+        kwargs.setdefault("weights_filling", "constant")
+        kwargs.setdefault("weights_stddev", 1.0)
+        kwargs.setdefault("bias_stddev", 0.0)
+        super(LayerNormForward, self).__init__(workflow, **kwargs)
+        self.eps = kwargs.get("eps", 1e-5)
+        if not 0 <= self.eps < 1e30:
+            raise ValueError("layer_norm: eps is %r" % (self.eps,))
+        self.mean = Array()
+        self.rstd = Array()
+
+    def initialize(self, device=None, **kwargs):
+        super(LayerNormForward, self).initialize(device=device, **kwargs)
+        if self.input is None or not self.input:
+            return False
+        if len(self.input.shape) < 2:
+            raise ValueError("layer_norm: input shape %s has no features" %
+                             (self.input.shape,))
+        C = self.input.shape[-1]
+        rows = self.input.size // C
+        if not self.weights:
+            self.weights.mem = numpy.zeros(C, numpy.float32)
+            self.fill_array(self.weights_filling, self.weights,
+                            self.weights_stddev)
+        if self.include_bias and not self.bias:
+            self.bias.mem = numpy.zeros(C, numpy.float32)
+            self.fill_array(self.bias_filling, self.bias, self.bias_stddev)
+        if not self.output or self.output.shape != self.input.shape:
+            self.output.reset(numpy.zeros(self.input.shape,
+                                          numpy.float32))
+            self.output.device_dtype = "bf16"
+        for arr in (self.mean, self.rstd):
+            if not arr or arr.shape != (rows,):
+                arr.reset(numpy.zeros(rows, numpy.float32))
+            self.init_array(arr, device_dtype="f32")
+        self.init_array(self.weights, device_dtype="f32")
+        if self.include_bias:
+            self.init_array(self.bias, device_dtype="f32")
+        self.init_array(self.output)
+
+    def numpy_run(self):
+        self.input.map_read()
+        for arr in (self.output, self.mean, self.rstd):
+            arr.map_invalidate()
+        x = self.input.mem.reshape(-1, self.input.shape[-1])
+        mean = x.mean(axis=1, keepdims=True)
+        xc = x - mean
+        rstd = 1.0 / numpy.sqrt((xc * xc).mean(axis=1, keepdims=True) +
+                                self.eps)
+        y = xc * rstd * self.weights.mem
+        if self.include_bias:
+            y = y + self.bias.mem
+        self.mean.mem[...] = mean[:, 0]
+        self.rstd.mem[...] = rstd[:, 0]
+        self.output.mem[...] = y.reshape(self.output.shape)
+
+    def hip_run(self):
+        from veles.znicz_amd import ops
+        train = not self.forward_mode
+        ops.layer_norm_fwd(
+            self.input.devmem, self.output.devmem, self.weights.devmem,
+            self.bias.devmem if self.include_bias else None,
+            self.mean.devmem if train else None,
+            self.rstd.devmem if train else None, self.eps)
+        self.output.touch_device()
+        if train:
+            self.mean.touch_device()
+            self.rstd.touch_device()
+
+
+class LayerNormBackward(GradientDescentBase):
+    """err_input and the gradients of the gain and the bias in one pass over
+    err_output and input; the update is that of the fully-connected layers
+    (batch mean, decay, momentum, the reducer's buckets)."""
+
+    MAPPING = "layer_norm"
+    BACKWARD = True
+    LINK_FROM_FORWARD = ("mean", "rstd")
+
+    def __init__(self, workflow, **kwargs):
+        super(LayerNormBackward, self).__init__(workflow, **kwargs)
+        self.mean = None            # linked
+        self.rstd = None
+        self.forward_unit = None
+
+    def initialize(self, device=None, **kwargs):
+        if self.err_output is None or not self.err_output:
+            return False
+        if self.input is None or not self.input:
+            return False
+        if self.need_err_input and (
+                not self.err_input or
+                self.err_input.shape != self.input.shape):
+            self.err_input.reset(numpy.zeros(self.input.shape,
+                                             numpy.float32))
+            self.err_input.device_dtype = "bf16"
+        super(LayerNormBackward, self).initialize(device=device, **kwargs)
+        if self.need_err_input:
+            self.init_array(self.err_input)
+
+    def numpy_run(self):
+        for arr in (self.err_output, self.input, self.mean, self.rstd):
+            arr.map_read()
+        C = self.input.shape[-1]
+        x = self.input.mem.reshape(-1, C)
+        dy = self.err_output.mem.reshape(-1, C)
+        rstd = self.rstd.mem[:, None]
+        xh = (x - self.mean.mem[:, None]) * rstd
+        gw, gb = (dy * xh).sum(axis=0), dy.sum(axis=0)
+        if self.need_err_input:
+            self.err_input.map_invalidate()
+            g = dy * self.weights.mem
+            dx = rstd * (g - g.mean(axis=1, keepdims=True) -
+                         xh * (g * xh).mean(axis=1, keepdims=True))
+            self.err_input.mem[...] = dx.reshape(self.err_input.shape)
+        self.numpy_update_weights(gw)
+        self.numpy_update_bias(gb)
+
+    def hip_run(self):
+        from veles.znicz_amd import ops
+        has_bias = self.include_bias and self.bias is not None and \
+            bool(self.bias)
+        shape = self.input.devmem.shape
+        ops.layer_norm_bwd(
+            self.err_output.devmem.view(shape), self.input.devmem,
+            self.weights.devmem, self.mean.devmem, self.rstd.devmem,
+            self.err_input.devmem if self.need_err_input else None,
+            self.gradient_weights.devmem,
+            self.gradient_bias.devmem if has_bias else None,
+            accumulate=self.accumulate_gradient)
+        if self.need_err_input:
+            self.err_input.touch_device()
+        self.gradient_weights.touch_device()
+        if has_bias:
+            self.gradient_bias.touch_device()
+        self._hip_apply(self.err_output.shape[0])

@@ -298,6 +298,58 @@ def histogram(x, counts, lo, hi):
     require().histogram(x, counts, float(lo), float(hi))
 
 
+def _rows(t):
+    """2-D view of a tensor's rows (its last dimension), without a copy."""
+    return t if t.dim() == 2 else t.view(-1, t.shape[-1])
+
+
+def token_logprobs(logits, labels=None, logprob=None, entropy=None,
+                   top_idx=None, top_logprob=None, batch=None):
+    """Answers of rows of logits [..., V] (bf16, fp16 or fp32; rows
+    contiguous, any stride apart), each output optional:
+
+    * ``logprob`` fp32[rows]: log probability of ``labels`` int32[rows].  A
+      label below 0 is none (0 is written); one of V or more gives NaN.
+    * ``entropy`` fp32[rows], in nats.
+    * ``top_idx`` int32[rows, K], ``top_logprob`` fp32[rows, K], K at most
+      128: the likeliest classes, of equal ones the lower first.  Places
+      without a class hold -1 and minus infinity.
+
+    A logit of minus infinity forbids its class; a row of them has entropy 0
+    and log probabilities of minus infinity.  A row with NaN or plus infinity
+    gives NaN, and -1 for its classes.  Rows from ``batch`` on are padding:
+    they are not read, and hold zeros (``top_idx`` -1)."""
+    x = _rows(logits)
+    require().token_logprobs(x, labels, logprob, entropy, top_idx,
+                             top_logprob,
+                             x.shape[0] if batch is None else int(batch))
+
+
+def eval_distill(logits, top_idx, top_logit, err_out, loss=None, batch=None,
+                 temperature=1.0, labels=None, n_err=None):
+    """Distillation of a student's ``logits`` [..., V] from a teacher's top
+    classes ``top_idx`` int32[rows, K] and their logits or log probabilities
+    ``top_logit`` fp32[rows, K] (K at most 128), at ``temperature`` t:
+
+        q = softmax(top_logit / t),  p = softmax(logits / t)
+        loss = t^2 sum q (ln q - ln p)       fp32[rows]
+        err_out = d loss / d logits = t (p - q)
+
+    ``err_out`` has the logits' type and shape and may be ``logits`` itself;
+    that of fp32 logits may be bf16.
+    Places with a negative class or a logit of minus infinity are empty; a
+    class that is named twice has both shares.  A row without a named class,
+    or whose logits are all minus infinity, has no loss and no gradient; one
+    with NaN, plus infinity or a class of V or more gives NaN.  Rows from
+    ``batch`` on are padding and hold zeros.  With ``labels`` int32[rows],
+    ``n_err[0]`` (int32) grows by the rows whose likeliest class is another
+    (labels below 0 are none)."""
+    x = _rows(logits)
+    require().eval_distill(x, top_idx, top_logit, _rows(err_out), loss,
+                           x.shape[0] if batch is None else int(batch),
+                           float(temperature), labels, n_err)
+
+
 def eval_mse(y, target, err_out, mse, metrics, batch, root):
     require().eval_mse(y, target, err_out, mse, metrics, int(batch),
                        int(root))
@@ -343,6 +395,27 @@ def lrn_fwd(x, out, denom, alpha, beta, k, n):
 def lrn_bwd(err_out, x, out, denom, err_in, alpha, beta, k, n):
     require().lrn_bwd(err_out, x, out, denom, err_in, float(alpha),
                       float(beta), float(k), int(n))
+
+
+def layer_norm_fwd(x, out, weights, bias, mean, rstd, eps=1e-5):
+    """out = (x - mean) rstd * weights + bias over the last dimension.
+
+    x, out: bf16, fp16 or fp32, rows contiguous, any stride apart; ``out``
+    may be ``x``.  weights, bias: fp32[C] or None; mean, rstd: fp32[rows],
+    written for the backward pass, or None."""
+    require().layer_norm_fwd(_rows(x), _rows(out), weights, bias, mean,
+                             rstd, float(eps))
+
+
+def layer_norm_bwd(err_out, x, weights, mean, rstd, err_in, grad_w=None,
+                   grad_b=None, accumulate=False):
+    """Backward of :func:`layer_norm_fwd` with the ``mean`` and ``rstd`` it
+    wrote.  err_in (or None) may be ``err_out`` or ``x``; grad_w, grad_b:
+    fp32[C] or None, sums over all rows, always in the same order
+    (``accumulate``: added to what they hold)."""
+    require().layer_norm_bwd(_rows(err_out), _rows(x), weights, mean, rstd,
+                             None if err_in is None else _rows(err_in),
+                             grad_w, grad_b, bool(accumulate))
 
 
 def dropout_fwd(x, out, mask, ratio, seed, counter, ctr_buf=None):

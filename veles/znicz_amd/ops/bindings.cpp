@@ -81,6 +81,19 @@ void lrn_fwd_launch(const unsigned short*, unsigned short*, float*, long,
 void lrn_bwd_launch(const unsigned short*, const unsigned short*,
                     const float*, float*, unsigned short*, long, int,
                     float, float, float, int, hipStream_t);
+// from layer_norm.hip
+void layer_norm_fwd_launch(int, RowsIn, RowsOut, const float*, const float*,
+                           float*, float*, long, int, float, hipStream_t);
+long layer_norm_bwd_scratch(int, long, int);
+void layer_norm_bwd_launch(int, RowsIn, RowsIn, const float*, const float*,
+                           const float*, RowsOut, float*, float*, bool,
+                           float*, long, int, hipStream_t);
+// from token_probs.hip
+void token_logprobs_launch(int, RowsIn, const int*, float*, float*, int*,
+                           float*, int, long, long, int, hipStream_t);
+void eval_distill_launch(int, int, RowsIn, const int*, const float*, RowsOut,
+                         float*, const int*, int*, int, long, long, int,
+                         float, hipStream_t);
 
 namespace {
 
@@ -462,6 +475,222 @@ void confusion_accum(torch::Tensor max_idx, torch::Tensor labels,
                    cur_stream());
 }
 
+// -- row-wise operators (layer_norm.hip, token_probs.hip) -------------------
+// Matrices [rows, cols] of bf16, fp16 or fp32 whose rows are contiguous, any
+// stride apart; everything else contiguous.
+
+using Opt = c10::optional<torch::Tensor>;
+
+int row_type(const char* op, const torch::Tensor& t) {
+  switch (t.scalar_type()) {
+    case torch::kBFloat16: return ROW_BF16;
+    case torch::kFloat16: return ROW_F16;
+    case torch::kFloat32: return ROW_F32;
+    default:
+      TORCH_CHECK(false, op, ": expected bf16, fp16 or fp32, got ",
+                  t.scalar_type());
+  }
+}
+
+void check_rows(const char* op, const char* name, const torch::Tensor& t,
+                const torch::Tensor& like, at::ScalarType type,
+                bool written) {
+  TORCH_CHECK(t.device() == like.device(), op, ": ", name, " is on ",
+              t.device(), ", not on ", like.device());
+  TORCH_CHECK(t.scalar_type() == type, op, ": ", name, " is ",
+              t.scalar_type(), ", not ", type);
+  TORCH_CHECK(t.dim() == 2, op, ": ", name, " must have 2 dimensions");
+  TORCH_CHECK(t.sizes() == like.sizes(), op, ": ", name, " is ", t.sizes(),
+              ", not ", like.sizes());
+  TORCH_CHECK(t.size(1) > 0, op, ": rows of no columns");
+  TORCH_CHECK(t.size(1) < (1ll << 30), op, ": rows of 2^30 columns or more");
+  TORCH_CHECK(t.size(1) == 1 || t.stride(1) == 1, op, ": the rows of ", name,
+              " must be contiguous");
+  if (written)
+    TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), op,
+                ": the rows of ", name, " overlap");
+}
+
+// an array of n numbers, or nothing
+template <typename V>
+V* array(const char* op, const char* name, const Opt& t, int64_t n,
+         const torch::Tensor& like) {
+  if (!t.has_value()) return nullptr;
+  TORCH_CHECK(t->device() == like.device(), op, ": ", name, " is on ",
+              t->device(), ", not on ", like.device());
+  TORCH_CHECK(t->scalar_type() == c10::CppTypeToScalarType<V>::value, op,
+              ": ", name, " is ", t->scalar_type(), ", not ",
+              c10::CppTypeToScalarType<V>::value);
+  TORCH_CHECK(t->is_contiguous(), op, ": ", name, " must be contiguous");
+  TORCH_CHECK(t->numel() == n, op, ": ", name, " has ", t->numel(),
+              " elements, not ", n);
+  return t->data_ptr<V>();
+}
+
+RowsIn rows_in(const torch::Tensor& t) {
+  return RowsIn{t.data_ptr(), (long)t.stride(0)};
+}
+
+RowsOut rows_out(const torch::Tensor& t) {
+  return RowsOut{t.data_ptr(), (long)t.stride(0)};
+}
+
+// (the last check of all, so that the others hold without a GPU too)
+void check_gpu(const char* op, const torch::Tensor& x) {
+  TORCH_CHECK(x.is_cuda(), op, ": the tensors are not on a GPU");
+}
+
+// An output may be an input itself, element for element, or lie between its
+// rows, but not over a part of it.
+void check_overlap(const char* op, const char* name, const torch::Tensor& out,
+                   const torch::Tensor& in) {
+  const int64_t R = out.size(0), C = out.size(1);
+  if (R == 0) return;
+  const int64_t so = R == 1 ? 0 : out.stride(0) * out.element_size();
+  const int64_t si = R == 1 ? 0 : in.stride(0) * in.element_size();
+  const int64_t wo = C * out.element_size(), wi = C * in.element_size();
+  const char* po = static_cast<const char*>(out.data_ptr());
+  const char* pi = static_cast<const char*>(in.data_ptr());
+  bool over = po < pi + (R - 1) * si + wi && pi < po + (R - 1) * so + wo;
+  if (over && so == si && wo == wi && po == pi) over = false;
+  if (over && so == si && so > 0) {
+    const int64_t d = ((pi - po) % so + so) % so;   // in's rows after out's
+    over = d < wo || so - d < wi;
+  }
+  TORCH_CHECK(!over, op, ": ", name, " overlaps an input in part");
+}
+
+void layer_norm_fwd(torch::Tensor x, torch::Tensor y, Opt w, Opt b, Opt mean,
+                    Opt rstd, double eps) {
+  const char* op = "layer_norm_fwd";
+  check_rows(op, "x", x, x, x.scalar_type(), false);
+  check_rows(op, "out", y, x, x.scalar_type(), true);
+  check_overlap(op, "out", y, x);
+  TORCH_CHECK(eps >= 0 && eps < 1e30, op, ": eps is ", eps);
+  const int type = row_type(op, x);
+  const int64_t R = x.size(0), C = x.size(1);
+  const float* wp = array<float>(op, "weights", w, C, x);
+  const float* bp = array<float>(op, "bias", b, C, x);
+  float* mp = array<float>(op, "mean", mean, R, x);
+  float* rp = array<float>(op, "rstd", rstd, R, x);
+  check_gpu(op, x);
+  c10::DeviceGuard guard(x.device());
+  layer_norm_fwd_launch(type, rows_in(x), rows_out(y), wp, bp, mp, rp, R,
+                        (int)C, (float)eps, cur_stream());
+}
+
+void layer_norm_bwd(torch::Tensor dy, torch::Tensor x, Opt w,
+                    torch::Tensor mean, torch::Tensor rstd, Opt dx, Opt dw,
+                    Opt db, bool accumulate) {
+  const char* op = "layer_norm_bwd";
+  check_rows(op, "x", x, x, x.scalar_type(), false);
+  check_rows(op, "err_output", dy, x, x.scalar_type(), false);
+  RowsOut out{nullptr, 0};
+  if (dx.has_value()) {
+    check_rows(op, "err_input", *dx, x, x.scalar_type(), true);
+    check_overlap(op, "err_input", *dx, x);
+    check_overlap(op, "err_input", *dx, dy);
+    out = rows_out(*dx);
+  }
+  const int type = row_type(op, x);
+  const int64_t R = x.size(0), C = x.size(1);
+  const float* wp = array<float>(op, "weights", w, C, x);
+  const float* mp = array<float>(op, "mean", mean, R, x);
+  const float* rp = array<float>(op, "rstd", rstd, R, x);
+  float* dwp = array<float>(op, "grad_w", dw, C, x);
+  float* dbp = array<float>(op, "grad_b", db, C, x);
+  check_gpu(op, x);
+  c10::DeviceGuard guard(x.device());
+  torch::Tensor part;
+  float* pp = nullptr;
+  const long n = dwp || dbp ? layer_norm_bwd_scratch(type, R, (int)C) : 0;
+  if (n) {
+    part = torch::empty({n}, x.options().dtype(torch::kFloat32));
+    pp = part.data_ptr<float>();
+  }
+  layer_norm_bwd_launch(type, rows_in(dy), rows_in(x), wp, mp, rp, out, dwp,
+                        dbp, accumulate, pp, R, (int)C, cur_stream());
+}
+
+int64_t live_rows(const char* op, int64_t batch, int64_t rows) {
+  TORCH_CHECK(batch >= 0 && batch <= rows, op, ": batch is ", batch, " of ",
+              rows, " rows");
+  return batch;
+}
+
+void token_logprobs(torch::Tensor x, Opt labels, Opt logprob, Opt entropy,
+                    Opt top_idx, Opt top_lp, int64_t batch) {
+  const char* op = "token_logprobs";
+  check_rows(op, "logits", x, x, x.scalar_type(), false);
+  const int type = row_type(op, x);
+  const int64_t R = x.size(0), C = x.size(1);
+  const int64_t live = live_rows(op, batch, R);
+  TORCH_CHECK(logprob.has_value() == labels.has_value(), op,
+              ": labels and logprob come together");
+  TORCH_CHECK(top_idx.has_value() == top_lp.has_value(), op,
+              ": top_idx and top_logprob come together");
+  int64_t top = 0;
+  if (top_idx.has_value()) {
+    TORCH_CHECK(top_idx->dim() == 2 && top_idx->size(0) == R, op,
+                ": top_idx must be [", R, ", top]");
+    TORCH_CHECK(top_idx->sizes() == top_lp->sizes(), op,
+                ": top_logprob is ", top_lp->sizes(), ", not ",
+                top_idx->sizes());
+    top = top_idx->size(1);
+    TORCH_CHECK(top <= MAX_TOP, op, ": ", top, " alternatives of at most ",
+                MAX_TOP);
+  }
+  const int* lp = array<int>(op, "labels", labels, R, x);
+  float* gp = array<float>(op, "logprob", logprob, R, x);
+  float* ep = array<float>(op, "entropy", entropy, R, x);
+  int* ip = array<int>(op, "top_idx", top_idx, R * top, x);
+  float* tp = array<float>(op, "top_logprob", top_lp, R * top, x);
+  check_gpu(op, x);
+  c10::DeviceGuard guard(x.device());
+  token_logprobs_launch(type, rows_in(x), lp, gp, ep, ip, tp, (int)top, R,
+                        live, (int)C, cur_stream());
+}
+
+void eval_distill(torch::Tensor x, torch::Tensor idx, torch::Tensor z,
+                  torch::Tensor err, Opt loss, int64_t batch, double tau,
+                  Opt labels, Opt n_err) {
+  const char* op = "eval_distill";
+  check_rows(op, "logits", x, x, x.scalar_type(), false);
+  const int type = row_type(op, x);
+  // fp32 logits may have a bf16 gradient, which is what GD units take
+  const bool narrow = type == ROW_F32 &&
+                      err.scalar_type() == torch::kBFloat16;
+  check_rows(op, "err_output", err, x,
+             narrow ? torch::kBFloat16 : x.scalar_type(), true);
+  check_overlap(op, "err_output", err, x);
+  const int64_t R = x.size(0), C = x.size(1);
+  const int64_t live = live_rows(op, batch, R);
+  TORCH_CHECK(tau >= 1e-3 && tau <= 1e3, op, ": temperature is ", tau,
+              ", not within 0.001 and 1000");
+  TORCH_CHECK(idx.dim() == 2 && idx.size(0) == R, op, ": top_idx must be [",
+              R, ", top]");
+  TORCH_CHECK(z.sizes() == idx.sizes(), op, ": top_logit is ", z.sizes(),
+              ", not ", idx.sizes());
+  const int64_t top = idx.size(1);
+  TORCH_CHECK(top >= 1 && top <= MAX_TOP, op, ": ", top,
+              " teacher's classes, not 1 to ", MAX_TOP);
+  TORCH_CHECK(labels.has_value() == n_err.has_value(), op,
+              ": labels and n_err come together");
+  if (n_err.has_value())
+    TORCH_CHECK(n_err->numel() >= 1, op, ": n_err is empty");
+  const int* ip = array<int>(op, "top_idx", idx, R * top, x);
+  const float* zp = array<float>(op, "top_logit", z, R * top, x);
+  float* sp = array<float>(op, "loss", loss, R, x);
+  const int* lp = array<int>(op, "labels", labels, R, x);
+  int* np = array<int>(op, "n_err", n_err,
+                       n_err.has_value() ? n_err->numel() : 0, x);
+  check_gpu(op, x);
+  c10::DeviceGuard guard(x.device());
+  eval_distill_launch(type, narrow ? ROW_BF16 : type, rows_in(x), ip, zp,
+                      rows_out(err), sp, lp, np, (int)top, R, live, (int)C,
+                      (float)tau, cur_stream());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -503,6 +732,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dropout_fwd", &dropout_fwd);
   m.def("dropout_bwd", &dropout_bwd);
   m.def("histogram", &histogram, "LDS histogram (counts int32)");
+  m.def("layer_norm_fwd", &layer_norm_fwd);
+  m.def("layer_norm_bwd", &layer_norm_bwd);
+  m.def("token_logprobs", &token_logprobs);
+  m.def("eval_distill", &eval_distill);
   m.def("set_routing", &set_routing_py,
         "override GEMM routing constants (gfx950_routing.json)");
   m.def("set_fc_split", &set_fc_split_py,

@@ -57,3 +57,19 @@ struct PoolDesc {
   int OH, OW;
   unsigned long long seed;   // for stochastic pooling
 };
+
+// element types of the row-wise kernels (layer_norm.hip, token_probs.hip)
+enum RowType { ROW_BF16 = 0, ROW_F16 = 1, ROW_F32 = 2 };
+
+// A matrix in memory: rows of contiguous elements, `stride` elements apart
+struct RowsIn {
+  const void* p;
+  long stride;
+};
+struct RowsOut {
+  void* p;
+  long stride;
+};
+
+// most top classes of a row (token_logprobs, eval_distill)
+#define MAX_TOP 128

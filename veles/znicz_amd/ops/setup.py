@@ -26,6 +26,8 @@ ext = CUDAExtension(
         "hip/elementwise.hip",
         "hip/softmax.hip",
         "hip/pool_lrn.hip",
+        "hip/layer_norm.hip",
+        "hip/token_probs.hip",
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],

@@ -13,6 +13,8 @@ kwargs}, "<-": {gd kwargs}, ...shared kwargs...}``.
 
 from veles.units import Unit
 from veles.znicz_amd.decision import DecisionGD, DecisionMSE
+from veles.znicz_amd.distillation import EvaluatorDistillation, \
+    TeacherAnswers
 from veles.znicz_amd.evaluator import EvaluatorSoftmax, EvaluatorMSE
 from veles.znicz_amd.nn_units import (
     MatchingObject, NNSnapshotter, NNWorkflow)
@@ -49,6 +51,9 @@ class StandardWorkflowBase(NNWorkflow):
         self.decision_config = kwargs.pop("decision_config", {})
         self.snapshotter_config = kwargs.pop("snapshotter_config", {})
         self.loss_function = kwargs.pop("loss_function", "softmax")
+        #: loss_function "distillation": {"snapshot": teacher's file, "top":
+        #: classes of it for each sample, "temperature": ...}
+        self.distillation_config = kwargs.pop("distillation_config", {})
         super(StandardWorkflowBase, self).__init__(workflow, **kwargs)
 
     # -- layer parsing ------------------------------------------------------
@@ -145,25 +150,48 @@ class StandardWorkflow(StandardWorkflowBase):
             self.evaluator.link_attrs(
                 self.loader, ("target", "minibatch_targets"),
                 ("batch_size", "minibatch_size"))
+        elif self.loss_function == "distillation":
+            parents = (self.link_teacher(*parents),)
+            if hasattr(self.forwards[-1], "logits_only"):
+                self.forwards[-1].logits_only = True
+            self.evaluator = EvaluatorDistillation(
+                self, **self.distillation_config)
+            self.evaluator.teacher = self.teacher
+            self.evaluator.link_attrs(self.forwards[-1],
+                                      ("input", "output"))
+            self.evaluator.link_attrs(
+                self.teacher, "top_idx", ("top_logit", "top_logprob"))
+            self.evaluator.link_attrs(
+                self.loader, ("labels", "minibatch_labels"),
+                ("batch_size", "minibatch_size"))
         else:
-            raise ValueError("loss_function must be softmax|mse")
+            raise ValueError(
+                "loss_function must be softmax|mse|distillation")
         self.evaluator.link_from(*parents)
         return self.evaluator
 
+    def link_teacher(self, *parents):
+        self.teacher = TeacherAnswers(self, **self.distillation_config)
+        self.teacher.link_attrs(
+            self.loader, ("input", "minibatch_data"),
+            ("batch_size", "minibatch_size"))
+        self.teacher.link_from(*parents)
+        return self.teacher
+
     def link_decision(self, *parents):
-        cls = DecisionGD if self.loss_function == "softmax" else DecisionMSE
+        cls = DecisionMSE if self.loss_function == "mse" else DecisionGD
         self.decision = cls(self, **self.decision_config)
         self.decision.link_from(*parents)
         self.decision.link_attrs(
             self.loader, "minibatch_class", "minibatch_size",
             "last_minibatch", "class_lengths", "epoch_ended",
             "epoch_number")
-        if self.loss_function == "softmax":
-            self.decision.link_attrs(self.evaluator,
-                                     ("minibatch_n_err", "n_err"))
-        else:
+        if self.loss_function == "mse":
             self.decision.link_attrs(self.evaluator,
                                      ("minibatch_metrics", "metrics"))
+        else:
+            self.decision.link_attrs(self.evaluator,
+                                     ("minibatch_n_err", "n_err"))
         self.decision.evaluator = self.evaluator
         return self.decision
 
