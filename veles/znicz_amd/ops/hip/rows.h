@@ -1,6 +1,8 @@
 // What the row-wise kernels share (layer_norm.hip, token_probs.hip): the
 // element types, and sums and maxima over a wave and a workgroup.
 #pragma once
+#include <hip/hip_runtime.h>
+
 #include "common.h"
 
 typedef __bf16 bf16_t;
