@@ -89,8 +89,10 @@ void layer_norm_bwd_launch(int, RowsIn, RowsIn, const float*, const float*,
                            const float*, RowsOut, float*, float*, bool,
                            float*, long, int, hipStream_t);
 // from token_probs.hip
+long token_logprobs_scratch(int, long, int, int);
 void token_logprobs_launch(int, RowsIn, const int*, float*, float*, int*,
-                           float*, int, long, long, int, hipStream_t);
+                           float*, int, long, long, int, void*,
+                           hipStream_t);
 void eval_distill_launch(int, int, RowsIn, const int*, const float*, RowsOut,
                          float*, const int*, int*, int, long, long, int,
                          float, hipStream_t);
@@ -647,8 +649,15 @@ void token_logprobs(torch::Tensor x, Opt labels, Opt logprob, Opt entropy,
   float* tp = array<float>(op, "top_logprob", top_lp, R * top, x);
   check_gpu(op, x);
   c10::DeviceGuard guard(x.device());
+  torch::Tensor scratch;
+  void* sp = nullptr;
+  const long n = token_logprobs_scratch(type, live, (int)C, (int)top);
+  if (n) {
+    scratch = torch::empty({n}, x.options().dtype(torch::kUInt8));
+    sp = scratch.data_ptr();
+  }
   token_logprobs_launch(type, rows_in(x), lp, gp, ep, ip, tp, (int)top, R,
-                        live, (int)C, cur_stream());
+                        live, (int)C, sp, cur_stream());
 }
 
 void eval_distill(torch::Tensor x, torch::Tensor idx, torch::Tensor z,

@@ -50,6 +50,45 @@ __device__ __forceinline__ float block_max(float v, float* tmp) {
   return v;
 }
 
+// 16 bytes of a row.  A row may begin at any element, so these loads and
+// stores ask for no more than an element's alignment.
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+
+template <typename T>
+struct Pack {
+  static constexpr int N = 16 / sizeof(T);
+  u32x4 raw;
+
+  __device__ __forceinline__ void load(const T* p) {
+    __builtin_memcpy(&raw, p, 16);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    __builtin_memcpy(p, &raw, 16);
+  }
+  // The compiler forgets what it knows of the elements, so that it takes
+  // them apart again where they are used again, instead of holding them in
+  // 32 bits each from one use to the other.
+  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(raw)); }
+  __device__ __forceinline__ void fill(float v) {
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = from_f<T>(v);
+    __builtin_memcpy(&raw, t, 16);
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    T t[N];
+    __builtin_memcpy(t, &raw, 16);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (float)t[i];
+  }
+  __device__ __forceinline__ void set(const float* v) {
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = from_f<T>(v[i]);
+    __builtin_memcpy(&raw, t, 16);
+  }
+};
+
 // one case for each element type; F is a macro of the type
 #define ROW_TYPE_SWITCH(code, F)                                             \
   switch (code) {                                                            \

@@ -17,36 +17,18 @@
 
 #include "rows.h"
 
-#define TP_THREADS 256
 #define LOG2E 1.44269504088896340736f
 #define LN2 0.69314718055994530942f
 // u is cut here where it is multiplied by its power, which is 0 by then
 #define U_MIN -200.f
-
-// largest allowed logit, and the sums over the row relative to it
-struct RowSums {
-  float m;      // -inf: no class is allowed
-  float um;     // C m, rounded, 0 for a row without classes
-  float d;      // C m - um
-  float s;      // sum 2^u; NaN: the row has a NaN or plus infinity
-  float w;      // sum 2^u u
-  bool far;     // u = (x - m) C
-};
-
-__device__ __forceinline__ void row_reference(RowSums& r, float c) {
-  const float m = r.m == -INFINITY ? 0.f : r.m;
-  r.um = m * c;
-  r.far = !(fabsf(r.um) < 0x1p20f);      // (d is below 1/16 then)
-  r.d = r.far ? 0.f : fmaf(m, c, -r.um);
-}
+// a thread's M is no lower, so that it stands for a thread without classes
+// too: 2^(M - M') of it and of any that counts is 0, and d is below 16
+#define M_MIN -0x1p28f
+// from here on u = (x - m) C (d is below 1/16 up to it)
+#define M_FAR 0x1p20f
 
 // (v_exp_f32, v_log_f32: one unit in the last place; powers below 2^-126
-// are 0, and the sums are 1 at least)
-template <bool FAR>
-__device__ __forceinline__ float exponent(float x, float c,
-                                          const RowSums& r) {
-  return FAR ? (x - r.m) * c : fmaf(x, c, -r.um);
-}
+// are 0, and the sums of a row are 1/2 at least)
 __device__ __forceinline__ float pow2(float u) {
   return __builtin_amdgcn_exp2f(u);
 }
@@ -54,10 +36,9 @@ __device__ __forceinline__ float log2_of(float s) {
   return __builtin_amdgcn_logf(s);
 }
 
-// ln of the sum of exp((x - m) / tau)
-__device__ __forceinline__ float ln_sum(const RowSums& r) {
-  return (log2_of(r.s) - r.d) * LN2;
-}
+// ---------------------------------------------------------------------------
+// order of classes
+// ---------------------------------------------------------------------------
 
 // an order of the values in whole numbers; the two zeros are one
 __device__ __forceinline__ int order_of(float x) {
@@ -67,122 +48,632 @@ __device__ __forceinline__ int order_of(float x) {
 __device__ __forceinline__ float value_of(int i) {
   return __int_as_float(i < 0 ? i ^ 0x7fffffff : i);
 }
+#define ORDER_NONE ((int)0x807fffff)    // of minus infinity
 
 // Value and class in one number: a larger value is first, of equal values
 // the lower class.  0 is below every class.
 typedef unsigned long long rank_t;
-__device__ __forceinline__ rank_t key_of(float x, int j) {
+__device__ __forceinline__ rank_t rank_of(float x, int j) {
   return ((rank_t)((unsigned)order_of(x) ^ 0x80000000u) << 32) |
          (unsigned)(0x7fffffff - j);
 }
-__device__ __forceinline__ float key_value(rank_t k) {
+__device__ __forceinline__ float rank_value(rank_t k) {
   return value_of((int)((unsigned)(k >> 32) ^ 0x80000000u));
 }
-__device__ __forceinline__ int key_class(rank_t k) {
+__device__ __forceinline__ int rank_class(rank_t k) {
   return 0x7fffffff - (int)(unsigned)k;
 }
 
-__device__ __forceinline__ rank_t block_max_key(rank_t v, rank_t* tmp) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) {
-    const rank_t o = __shfl_xor(v, off);
-    v = o > v ? o : v;
-  }
-  if ((threadIdx.x & (WAVE - 1)) == 0) tmp[threadIdx.x / WAVE] = v;
-  __syncthreads();
-  v = tmp[0];
-  for (int i = 1; i < (int)blockDim.x / WAVE; ++i) v = tmp[i] > v ? tmp[i] : v;
-  __syncthreads();
-  return v;
-}
+// ---------------------------------------------------------------------------
+// sums over a row
+// ---------------------------------------------------------------------------
 
-template <bool FAR, typename T>
-__device__ __forceinline__ void add_row(const T* x, int cols, float c,
-                                        const RowSums& r, float& s,
-                                        float& w) {
-  for (int j = threadIdx.x; j < cols; j += blockDim.x) {
-    const float u = exponent<FAR>((float)x[j], c, r);
+// largest logit and the sums relative to it
+struct Sums {
+  float m;      // -inf: no class is allowed
+  float um;     // M
+  float s;      // sum 2^u; NaN: the row has a NaN or plus infinity
+  float w;      // sum 2^u u (entropy alone)
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    um = M_MIN;
+    s = w = 0.f;
+  }
+  // the same sums to a larger m
+  __device__ __forceinline__ void raise(float to, float c) {
+    const float um2 = fmaxf(to * c, M_MIN);
+    const float by = um - um2, f = pow2(by);
+    w = f * fmaf(by, s, w);
+    s *= f;
+    m = to;
+    um = um2;
+  }
+  __device__ __forceinline__ void add(float x, float c) {
+    const float u = fmaf(x, c, -um);
     const float e = pow2(u);
     s += e;
     w = fmaf(e, fmaxf(u, U_MIN), w);
   }
+};
+
+// what a row's outputs are made of
+struct Row {
+  float m, c;
+  float um;      // of u = C x - um, unless `far`
+  bool far;
+  bool none;     // no class is allowed
+  bool bad;      // NaN or plus infinity
+  float s;       // sum 2^u
+  float ln;      // ln of the sum of exp((x - m) / tau)
+  float entropy;
+
+  __device__ __forceinline__ float u(float x) const {
+    return far ? (x - m) * c : fmaf(x, c, -um);
+  }
+  __device__ __forceinline__ void finish(const Sums& a, float c_) {
+    m = a.m;
+    c = c_;
+    um = a.um;
+    s = a.s;
+    far = !(fabsf(m * c) < M_FAR) && m != -INFINITY;
+    bad = s != s;
+    none = !bad && m == -INFINITY;
+    const float d = far ? 0.f : fmaf(m, c, -um);
+    ln = (log2_of(s) - d) * LN2;
+    entropy = none ? 0.f : (log2_of(s) - a.w / s) * LN2;
+  }
+};
+
+__device__ __forceinline__ bool is_far(float m, float c) {
+  return !(fabsf(m * c) < M_FAR) && m != -INFINITY;
 }
 
-template <typename T>
-__device__ RowSums row_sums(const T* x, int cols, float c, float* tmp) {
-  RowSums r;
+// the waves' sums joined, in every thread; `tmp`: one for each wave
+template <int THREADS>
+__device__ __forceinline__ Sums join_block(Sums a, float c, Sums* tmp) {
+  constexpr int WAVES = THREADS / WAVE;
+  a.raise(wave_max(a.m), c);
+  a.s = wave_sum(a.s);
+  a.w = wave_sum(a.w);
+  if (WAVES == 1) return a;
+  if ((threadIdx.x & (WAVE - 1)) == 0) tmp[threadIdx.x / WAVE] = a;
+  __syncthreads();
+  float m = tmp[0].m;
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) m = fmaxf(m, tmp[i].m);
+  Sums t;
+  t.clear();
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    Sums b = tmp[i];
+    b.raise(m, c);
+    t.m = b.m;
+    t.um = b.um;
+    t.s += b.s;
+    t.w += b.w;
+  }
+  return t;
+}
+
+// Sums of a part of a row, to the exact C m: parts are joined by
+// 2^((m - m') C)
+struct Part {
+  float m, s, w;
+  int first;     // lowest class with the value m
+};
+
+__device__ __forceinline__ Part part_of(const Sums& a, float c, int first) {
+  const float d = is_far(a.m, c) || a.m == -INFINITY
+                      ? 0.f : fmaf(a.m, c, -a.um);
+  const float f = pow2(-d);
+  return Part{a.m, f * a.s, f * fmaf(-d, a.s, a.w), first};
+}
+
+// n parts of a row joined, by every thread for itself
+__device__ __forceinline__ Row join_parts(const Part* p, int n, float c,
+                                          int* first) {
   float m = -INFINITY;
-  for (int j = threadIdx.x; j < cols; j += blockDim.x)
-    m = fmaxf(m, (float)x[j]);
-  r.m = block_max(m, tmp);
-  row_reference(r, c);
+  for (int i = 0; i < n; ++i) m = fmaxf(m, p[i].m);
   float s = 0.f, w = 0.f;
-  if (r.far)
-    add_row<true>(x, cols, c, r, s, w);
-  else
-    add_row<false>(x, cols, c, r, s, w);
-  r.s = block_sum(s, tmp);
-  r.w = block_sum(w, tmp);
+  int at = 0x7fffffff;
+  for (int i = 0; i < n; ++i) {
+    // (an empty part beside an empty row: no difference of infinities)
+    const float by = p[i].m == m ? 0.f : fmaxf((p[i].m - m) * c, M_MIN);
+    const float f = pow2(by);
+    s = fmaf(f, p[i].s, s);
+    w = fmaf(f, fmaf(by, p[i].s, p[i].w), w);
+    if (p[i].m == m) at = min(at, p[i].first);
+  }
+  Sums a;
+  a.m = m;
+  a.um = fmaxf(m * c, M_MIN);
+  a.s = s;
+  a.w = w;
+  Row r;
+  r.finish(a, c);
+  r.ln = log2_of(s) * LN2;               // (the parts are to the exact C m)
+  *first = at;
   return r;
 }
 
-// one workgroup to a row; the row is read again for each alternative
+// ---------------------------------------------------------------------------
+// a row, or a part of it, in the registers of a workgroup
+// ---------------------------------------------------------------------------
+
+// Thread t holds packs t, t + THREADS, ... and one of the last elements that
+// make no whole pack.  Places without an element hold minus infinity.
+template <typename T, int THREADS, int NV>
+struct Held {
+  static constexpr int N = Pack<T>::N;
+  static constexpr int MOST = THREADS * NV * N;
+  Pack<T> v[NV];
+  float rest;
+
+  __device__ __forceinline__ static int whole(int n) {
+    const int packs = n / N;
+    return packs < THREADS * NV ? packs : THREADS * NV;
+  }
+  // place of the element `rest`; those beyond it (a row longer than MOST)
+  // are left to the caller
+  __device__ __forceinline__ static int rest_at(int n) {
+    return n / N * N + threadIdx.x;
+  }
+
+  __device__ __forceinline__ void load(const T* x, int n) {
+    const int packs = whole(n);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int p = i * THREADS + threadIdx.x;
+      v[i].fill(-INFINITY);
+      // (one offset for all, from bases that are the same for a wave)
+      if (p < packs) v[i].load(x + i * THREADS * N + threadIdx.x * N);
+    }
+    const int j = rest_at(n);
+    rest = j < n ? (float)x[j] : -INFINITY;
+  }
+
+};
+
+// Packs are summed CHUNK at a time, relative to the thread's largest so far:
+// what follows a load of 16 bytes is done while the next ones are under way,
+// and no element is read twice.
+#define CHUNK 2
+
+template <typename T, int COUNT>
+__device__ __forceinline__ void add_packs(const Pack<T>* v, Sums& a, float c,
+                                          float* high) {
+  constexpr int N = Pack<T>::N;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    float e[N];
+    v[i].get(e);
+    float h = e[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) h = fmaxf(h, e[j]);
+    if (high) high[i] = h;
+    m = fmaxf(m, h);
+  }
+  a.raise(fmaxf(a.m, m), c);
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    float e[N];
+    v[i].get(e);
+#pragma unroll
+    for (int j = 0; j < N; ++j) a.add(e[j], c);
+  }
+}
+
+template <typename T, int THREADS, int NV>
+__device__ __forceinline__ Sums held_sums(const Held<T, THREADS, NV>& h,
+                                          int n, float c, float* high) {
+  constexpr int STEP = NV < CHUNK ? NV : CHUNK;
+  const int packs = h.whole(n);
+  Sums a;
+  a.clear();
+#pragma unroll
+  for (int i = 0; i < NV; i += STEP) {
+    if (i * THREADS >= packs) break;
+    add_packs<T, STEP>(h.v + i, a, c, high ? high + i : nullptr);
+  }
+  a.raise(fmaxf(a.m, h.rest), c);
+  a.add(h.rest, c);
+  return a;
+}
+
+// ---------------------------------------------------------------------------
+// token_logprobs
+// ---------------------------------------------------------------------------
+
+#define LP_THREADS 256
+// classes that may be looked at more closely; more of them (many equal
+// values) are thinned out first
+#define LP_CAND 512
+
+struct LogprobsOut {
+  const int* labels;
+  float* logprob;
+  float* entropy;
+  int* idx;
+  float* lp;
+  int top;
+};
+
+__device__ __forceinline__ void logprobs_padding(const LogprobsOut& o,
+                                                 long row) {
+  if (threadIdx.x == 0) {
+    if (o.logprob) o.logprob[row] = 0.f;
+    if (o.entropy) o.entropy[row] = 0.f;
+  }
+  for (int k = threadIdx.x; k < o.top; k += blockDim.x) {
+    o.idx[row * o.top + k] = -1;
+    o.lp[row * o.top + k] = 0.f;
+  }
+}
+
 template <typename T>
-__global__ __launch_bounds__(TP_THREADS) void logprobs_k(
-    RowsIn x_, const int* __restrict__ labels, float* __restrict__ logprob,
-    float* __restrict__ entropy, int* __restrict__ top_idx,
-    float* __restrict__ top_lp, int top, long rows, long live, int cols) {
-  __shared__ float tmp[TP_THREADS / WAVE];
-  __shared__ rank_t ktmp[TP_THREADS / WAVE];
+__device__ __forceinline__ void logprobs_row(const LogprobsOut& o, long row,
+                                             const T* x, int cols,
+                                             const Row& r) {
+  if (threadIdx.x) return;
+  if (o.entropy) o.entropy[row] = r.entropy;
+  if (o.logprob) {
+    const int l = o.labels[row];
+    float v = 0.f;
+    if (l >= cols)
+      v = NAN;
+    else if (l >= 0)
+      v = r.bad ? NAN : r.none ? -INFINITY : ((float)x[l] - r.m) - r.ln;
+    o.logprob[row] = v;
+  }
+}
+
+// the alternative of rank k; key 0: there is none
+__device__ __forceinline__ void logprobs_top(const LogprobsOut& o, long row,
+                                             int k, rank_t key,
+                                             const Row& r) {
+  o.idx[row * o.top + k] = key ? rank_class(key) : -1;
+  o.lp[row * o.top + k] =
+      r.bad ? NAN : key ? (rank_value(key) - r.m) - r.ln : -INFINITY;
+}
+
+template <int THREADS>
+__device__ __forceinline__ int block_count(int n, int* tmp) {
+  constexpr int WAVES = THREADS / WAVE;
+#pragma unroll
+  for (int off = 32; off; off >>= 1) n += __shfl_xor(n, off);
+  __syncthreads();
+  if ((threadIdx.x & (WAVE - 1)) == 0) tmp[threadIdx.x / WAVE] = n;
+  __syncthreads();
+  n = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) n += tmp[i];
+  return n;
+}
+
+// Among the threads' largest values, in `high`, one that at least `top` of
+// them reach, and not many more; by one wave.  All classes that reach it are
+// few, and the first `top` are among them.  Fewer than `top` threads with a
+// class: the lowest of all.
+template <int THREADS>
+__device__ __forceinline__ int find_bound(const int* high, int top) {
+  constexpr int PER = THREADS / WAVE;
+  int v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) v[i] = high[threadIdx.x + i * WAVE];
+  int hi = v[0];
+#pragma unroll
+  for (int i = 1; i < PER; ++i) hi = max(hi, v[i]);
+#pragma unroll
+  for (int off = 32; off; off >>= 1) hi = max(hi, __shfl_xor(hi, off));
+  int lo = ORDER_NONE + 1;
+  auto reach = [&](int b) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) n += __popcll(__ballot(v[i] >= b));
+    return n;
+  };
+  if (reach(lo) < top) return lo;
+  // reach(lo) >= top > reach(hi + 1)
+  while (lo < hi) {
+    const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) / 2u);
+    const int n = reach(mid);
+    if (n >= top) {
+      lo = mid;
+      if (n <= top + top / 4) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return lo;
+}
+
+template <int THREADS>
+struct TopSpace {
+  int high[THREADS];
+  rank_t cand[LP_CAND];
+  int n, bound;
+  int tmp[THREADS / WAVE];
+};
+
+// The `top` first classes of what the workgroup holds, as ranks in order in
+// cand[0..top); returns how many there are.  `high`: the largest value of
+// each pack of this thread.  Ends with all threads having their view of it.
+template <typename T, int THREADS, int NV>
+__device__ __forceinline__ int held_top(Held<T, THREADS, NV>& h, const T* x,
+                                        int n, int base, const float* high,
+                                        int top, TopSpace<THREADS>& sp,
+                                        rank_t* mine, int* place) {
+  constexpr int N = Pack<T>::N;
+  const int tid = threadIdx.x;
+  const int packs = h.whole(n);
+  if (tid < WAVE) {
+    const int b = find_bound<THREADS>(sp.high, top);
+    if (tid == 0) {
+      sp.bound = b;
+      sp.n = 0;
+    }
+  }
+  __syncthreads();
+  const float bound = value_of(sp.bound);
+  auto put = [&](float x, int j) {
+    if (x >= bound) {
+      const int at = atomicAdd(&sp.n, 1);
+      if (at < LP_CAND) sp.cand[at] = rank_of(x, base + j);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * THREADS >= packs) break;
+    if (high[i] >= bound) {
+      float e[N];
+      h.v[i].forget();
+      h.v[i].get(e);
+      const int p = (i * THREADS + tid) * N;
+#pragma unroll
+      for (int j = 0; j < N; ++j) put(e[j], p + j);
+    }
+  }
+  put(h.rest, h.rest_at(n));
+  __syncthreads();
+  int found = sp.n;
+  if (found > LP_CAND) {
+    // Too many reach the bound (one value many times): the top-th value
+    // itself, then among the classes that hold it the last that is needed,
+    // by halving; the part is read from the caches each time.
+    int lo = sp.bound, hi = 0x7f800000;
+    while (lo < hi) {
+      const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) / 2u);
+      int c = 0;
+      for (int j = tid; j < n; j += THREADS) c += order_of(x[j]) >= mid;
+      if (block_count<THREADS>(c, sp.tmp) >= top)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    int c = 0;
+    for (int j = tid; j < n; j += THREADS) c += order_of(x[j]) > lo;
+    const int need = top - block_count<THREADS>(c, sp.tmp);
+    int a = 0, b = n - 1;
+    while (a < b) {
+      const int mid = a + (b - a) / 2;
+      c = 0;
+      for (int j = tid; j <= mid; j += THREADS) c += order_of(x[j]) == lo;
+      if (block_count<THREADS>(c, sp.tmp) >= need)
+        b = mid;
+      else
+        a = mid + 1;
+    }
+    if (tid == 0) sp.n = 0;
+    __syncthreads();
+    for (int j = tid; j < n; j += THREADS) {
+      const int o = order_of(x[j]);
+      if (o > lo || (o == lo && j <= a))
+        sp.cand[atomicAdd(&sp.n, 1)] = rank_of(x[j], base + j);
+    }
+    __syncthreads();
+    found = sp.n;
+  }
+  // the place of each in the order is the number of those before it
+#pragma unroll
+  for (int i = 0; i * THREADS < LP_CAND; ++i) {
+    const int at = i * THREADS + tid;
+    mine[i] = at < found ? sp.cand[at] : 0;
+    int before = 0;
+    if (at < found)
+      for (int j = 0; j < found; ++j) before += sp.cand[j] > mine[i];
+    place[i] = before;
+  }
+  return found;
+}
+
+// One workgroup to a part of a row, which it holds in registers.  `parts`
+// null: it is the whole row, and the outputs are written; else its sums and
+// first classes, to be joined.
+template <typename T, int NV>
+__global__ __launch_bounds__(LP_THREADS) void logprobs_k(
+    RowsIn x_, LogprobsOut o, long rows, long live, int cols, int size,
+    Part* __restrict__ parts, rank_t* __restrict__ keys) {
+  __shared__ TopSpace<LP_THREADS> sp;
+  __shared__ Sums tmp[LP_THREADS / WAVE];
+  const int tid = threadIdx.x;
+  // (a grid of parts x rows, the rows in two dimensions)
+  const long row = (long)blockIdx.z * gridDim.y + blockIdx.y;
+  if (row >= rows) return;
+  const int seg = blockIdx.x;
+  const long item = row * gridDim.x + seg;
+  if (row >= live) {
+    logprobs_padding(o, row);
+    return;
+  }
+  const T* x = (const T*)x_.p + row * x_.stride;
+  const int base = seg * size;
+  const int n = min(size, cols - base);
+  Held<T, LP_THREADS, NV> h;
+  h.load(x + base, n);
+  float high[NV];
+  Sums a = held_sums(h, n, LOG2E, high);
+  sp.high[tid] = order_of(a.m);
+  a = join_block<LP_THREADS>(a, LOG2E, tmp);
+  if (is_far(a.m, LOG2E)) {
+    float s = 0.f, w = 0.f;
+    for (int j = tid; j < n; j += LP_THREADS) {
+      const float u = ((float)x[base + j] - a.m) * LOG2E, e = pow2(u);
+      s += e;
+      w = fmaf(e, fmaxf(u, U_MIN), w);
+    }
+    __syncthreads();
+    a.s = block_sum(s, (float*)tmp);
+    a.w = block_sum(w, (float*)tmp);
+  }
+  Row r;
+  r.finish(a, LOG2E);
+  if (parts) {
+    if (tid == 0) parts[item] = part_of(a, LOG2E, 0);
+  } else {
+    logprobs_row(o, row, x, cols, r);
+  }
+  if (!o.top) return;
+  rank_t mine[LP_CAND / LP_THREADS];
+  int place[LP_CAND / LP_THREADS], found = 0;
+  if (!r.bad && !r.none)
+    found = held_top(h, x + base, n, base, high, o.top, sp, mine, place);
+#pragma unroll
+  for (int i = 0; i < LP_CAND / LP_THREADS; ++i)
+    if (i * LP_THREADS + tid < found && place[i] < o.top) {
+      if (parts)
+        keys[item * o.top + place[i]] = mine[i];
+      else
+        logprobs_top(o, row, place[i], mine[i], r);
+    }
+  for (int k = found + tid; k < o.top; k += LP_THREADS) {
+    if (parts)
+      keys[item * o.top + k] = 0;
+    else
+      logprobs_top(o, row, k, 0, r);
+  }
+}
+
+// A row's parts joined.  Their classes are in order, so that the place of
+// one among all is found by halving each part's list.
+template <typename T>
+__global__ __launch_bounds__(LP_THREADS) void logprobs_join_k(
+    RowsIn x_, LogprobsOut o, const Part* __restrict__ parts,
+    const rank_t* __restrict__ keys, long rows, long live, int cols,
+    int split) {
+  extern __shared__ rank_t list[];
   for (long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int tid = threadIdx.x;
     if (row >= live) {
-      if (tid == 0) {
-        if (logprob) logprob[row] = 0.f;
-        if (entropy) entropy[row] = 0.f;
-      }
-      for (int k = tid; k < top; k += TP_THREADS) {
-        top_idx[row * top + k] = -1;
-        top_lp[row * top + k] = 0.f;
-      }
+      logprobs_padding(o, row);
       continue;
     }
     const T* x = (const T*)x_.p + row * x_.stride;
-    const RowSums r = row_sums(x, cols, LOG2E, tmp);
-    const bool none = r.m == -INFINITY && r.s == 0.f;
-    const bool bad = r.s != r.s;
-    const float ln = ln_sum(r);
-    if (tid == 0) {
-      if (entropy)
-        entropy[row] = none ? 0.f : (log2_of(r.s) - r.w / r.s) * LN2;
-      if (logprob) {
-        const int l = labels[row];
-        float v = 0.f;
-        if (l >= cols)
-          v = NAN;
-        else if (l >= 0)
-          v = bad ? NAN : none ? -INFINITY : ((float)x[l] - r.m) - ln;
-        logprob[row] = v;
+    const int all = split * o.top;
+    for (int i = threadIdx.x; i < all; i += LP_THREADS)
+      list[i] = keys[row * all + i];
+    int first;
+    const Row r = join_parts(parts + row * split, split, LOG2E, &first);
+    logprobs_row(o, row, x, cols, r);
+    __syncthreads();
+    if (r.bad || r.none) {
+      for (int k = threadIdx.x; k < o.top; k += LP_THREADS)
+        logprobs_top(o, row, k, 0, r);
+    } else {
+      for (int i = threadIdx.x; i < all; i += LP_THREADS) {
+        const rank_t key = list[i];
+        const int own = i / o.top;
+        // empty places come last, in the order of the list
+        int before = i - own * o.top;
+        for (int p = 0; p < split && before < o.top; ++p) {
+          if (p == own) continue;
+          int lo = 0, hi = o.top;        // the first that is not before it
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            const rank_t other = list[p * o.top + mid];
+            if (other > key || (other == key && p < own))
+              lo = mid + 1;
+            else
+              hi = mid;
+          }
+          before += lo;
+        }
+        if (before < o.top) logprobs_top(o, row, before, key, r);
       }
     }
+    __syncthreads();
+  }
+}
+
+// Rows of more classes than parts of registers are joined for: one
+// workgroup to a row, which is read again for each alternative.
+template <typename T>
+__global__ __launch_bounds__(LP_THREADS) void logprobs_long_k(
+    RowsIn x_, LogprobsOut o, long rows, long live, int cols) {
+  __shared__ Sums tmp[LP_THREADS / WAVE];
+  __shared__ rank_t ktmp[LP_THREADS / WAVE];
+  const int tid = threadIdx.x;
+  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+    if (row >= live) {
+      logprobs_padding(o, row);
+      continue;
+    }
+    const T* x = (const T*)x_.p + row * x_.stride;
+    float m = -INFINITY;
+    for (int j = tid; j < cols; j += LP_THREADS) m = fmaxf(m, (float)x[j]);
+    m = block_max(m, (float*)tmp);
+    const bool far = is_far(m, LOG2E);
+    Sums a;
+    a.clear();
+    a.m = m;
+    a.um = fmaxf(m * LOG2E, M_MIN);
+    for (int j = tid; j < cols; j += LP_THREADS) {
+      const float v = (float)x[j];
+      const float u = far ? (v - m) * LOG2E : fmaf(v, LOG2E, -a.um);
+      const float e = pow2(u);
+      a.s += e;
+      a.w = fmaf(e, fmaxf(u, U_MIN), a.w);
+    }
+    a.s = block_sum(a.s, (float*)tmp);
+    a.w = block_sum(a.w, (float*)tmp);
+    Row r;
+    r.finish(a, LOG2E);
+    logprobs_row(o, row, x, cols, r);
     rank_t last = ~0ull;
-    for (int k = 0; k < top; ++k) {
+    for (int k = 0; k < o.top; ++k) {
       rank_t best = 0;
-      if (!bad && !none && last)
-        for (int j = tid; j < cols; j += TP_THREADS) {
+      if (!r.bad && !r.none && last)
+        for (int j = tid; j < cols; j += LP_THREADS) {
           const float v = (float)x[j];
-          const rank_t key = v == -INFINITY ? 0 : key_of(v, j);
+          const rank_t key = v == -INFINITY ? 0 : rank_of(v, j);
           if (key < last && key > best) best = key;
         }
-      best = block_max_key(best, ktmp);
-      if (tid == 0) {
-        top_idx[row * top + k] = best ? key_class(best) : -1;
-        top_lp[row * top + k] =
-            bad ? NAN : best ? (key_value(best) - r.m) - ln : -INFINITY;
+#pragma unroll
+      for (int off = 32; off; off >>= 1) {
+        const rank_t other = __shfl_xor(best, off);
+        best = other > best ? other : best;
       }
+      if ((tid & (WAVE - 1)) == 0) ktmp[tid / WAVE] = best;
+      __syncthreads();
+      for (int i = 0; i < LP_THREADS / WAVE; ++i)
+        best = ktmp[i] > best ? ktmp[i] : best;
+      __syncthreads();
+      if (tid == 0) logprobs_top(o, row, k, best, r);
       last = best;
     }
   }
+}
+
+// ---------------------------------------------------------------------------
+// eval_distill
+// ---------------------------------------------------------------------------
+
+#define TP_THREADS 256
+
+__device__ __forceinline__ Row plain_row(const Sums& a, float c) {
+  Row r;
+  r.finish(a, c);
+  return r;
 }
 
 // Distillation: q = softmax(z / tau) over the teacher's classes, p =
@@ -208,8 +699,20 @@ __global__ __launch_bounds__(TP_THREADS) void distill_k(
     }
     const T* x = (const T*)x_.p + row * x_.stride;
     const float c = LOG2E / tau;
-    const RowSums r = row_sums(x, cols, c, tmp);
-    const bool none = r.m == -INFINITY && r.s == 0.f;
+    float m = -INFINITY;
+    for (int j = tid; j < cols; j += TP_THREADS) m = fmaxf(m, (float)x[j]);
+    m = block_max(m, tmp);
+    Sums sums;
+    sums.clear();
+    sums.m = m;
+    sums.um = fmaxf(m * c, M_MIN);
+    const bool far = is_far(m, c);
+    for (int j = tid; j < cols; j += TP_THREADS) {
+      const float v = (float)x[j];
+      sums.s += pow2(far ? (v - m) * c : fmaf(v, c, -sums.um));
+    }
+    sums.s = block_sum(sums.s, tmp);
+    const Row r = plain_row(sums, c);
     // the teacher's distribution: thread k has its k-th class
     int id = -1;
     float t = -INFINITY, xk = 0.f;
@@ -225,17 +728,17 @@ __global__ __launch_bounds__(TP_THREADS) void distill_k(
       }
       if (wrong || t == -INFINITY) id = -1;
     }
-    const bool bad = __syncthreads_or(wrong) || r.s != r.s;
+    const bool bad = __syncthreads_or(wrong) || r.bad;
     const float zm = block_max(id >= 0 ? t : -INFINITY, tmp);
     const float g = id >= 0 ? expf((t - zm) / tau) : 0.f;
     const float gs = block_sum(g, tmp);
-    const bool lost = none || zm == -INFINITY;
+    const bool lost = r.none || zm == -INFINITY;
     float q = 0.f, part = 0.f;
     if (!lost && id >= 0) {
       q = g / gs;
       // tau (ln q - ln p)
-      const float far = (t - zm) - (xk - r.m) + tau * (ln_sum(r) - logf(gs));
-      part = q > 0.f ? q * far : 0.f;
+      const float apart = (t - zm) - (xk - r.m) + tau * (r.ln - logf(gs));
+      part = q > 0.f ? q * apart : 0.f;
     }
     if (tid < top) {
       sid[tid] = id;
@@ -260,23 +763,20 @@ __global__ __launch_bounds__(TP_THREADS) void distill_k(
       if (tid == 0 && l >= 0) {
         for (int i = 1; i < TP_THREADS / WAVE; ++i)
           first = min(first, ((int*)tmp)[i]);
-        if (bad || none || first != l) atomicAdd(n_err, 1);
+        if (bad || r.none || first != l) atomicAdd(n_err, 1);
       }
     }
     // err may lie over x: what is read of x is read before
     float mine = 0.f, sum = 0.f;
     if (id >= 0) {
-      mine = r.far ? pow2(exponent<true>(xk, c, r))
-                   : pow2(exponent<false>(xk, c, r));
+      mine = pow2(r.u(xk));
       for (int k = 0; k < top; ++k)
         if (sid[k] == id) sum += sq[k];
     }
     __syncthreads();
     const float a = bad ? NAN : lost ? 0.f : tau / r.s;
     for (int j = tid; j < cols; j += TP_THREADS) {
-      const float v = (float)x[j];
-      const float e = r.far ? pow2(exponent<true>(v, c, r))
-                            : pow2(exponent<false>(v, c, r));
+      const float e = pow2(r.u((float)x[j]));
       err[j] = from_f<O>(lost && !bad ? 0.f : a * e);
     }
     __syncthreads();
@@ -290,24 +790,100 @@ static unsigned row_grid(long rows) {
   return (unsigned)(rows < 65536 ? rows : 65536);
 }
 
-void token_logprobs_launch(int type, RowsIn x, const int* labels,
-                           float* logprob, float* entropy, int* top_idx,
-                           float* top_lp, int top, long rows, long live,
-                           int cols, hipStream_t s) {
-  if (rows == 0) return;
-#define RUN(T)                                                               \
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_k<T>), dim3(row_grid(rows)),   \
-                     dim3(TP_THREADS), 0, s, x, labels, logprob, entropy,    \
-                     top_idx, top_lp, top, rows, live, cols)
-  ROW_TYPE_SWITCH(type, RUN)
-#undef RUN
+static dim3 parts_grid(int split, long rows) {
+  const long y = rows < 32768 ? rows : 32768;
+  return dim3((unsigned)split, (unsigned)y, (unsigned)((rows + y - 1) / y));
+}
+
+// parts of a row that are joined at most, and ranks of them in LDS
+#define LP_PARTS 64
+
+// How a call is laid out: packs of a thread, parts of a row
+struct LogprobsPlan {
+  int nv, split, size;
+};
+
+static LogprobsPlan logprobs_plan(int type, long rows, int cols) {
+  const int n = type == ROW_F32 ? 4 : 8;
+  const int most = LP_THREADS * 16 * n;
+  long split = (cols + most - 1) / most;
+  // few rows: parts of at least 4 packs a thread, up to two workgroups for
+  // each compute unit
+  const long least = LP_THREADS * 4 * n;
+  while (split < LP_PARTS && rows * split < 512 &&
+         cols / (split + 1) >= least)
+    ++split;
+  LogprobsPlan p;
+  p.split = (int)split;
+  // whole packs to a part
+  long size = (cols + split - 1) / split;
+  size = (size + n - 1) / n * n;
+  p.size = (int)size;
+  p.split = (int)((cols + size - 1) / size);
+  p.nv = 1;
+  while ((long)LP_THREADS * p.nv * n < size && p.nv < 16) p.nv *= 2;
+  return p;
+}
+
+// bytes that token_logprobs_launch needs at `scratch`
+long token_logprobs_scratch(int type, long live, int cols, int top) {
+  const LogprobsPlan p = logprobs_plan(type, live, cols);
+  if (p.split == 1 || p.split > LP_PARTS) return 0;
+  return live * p.split * ((long)sizeof(Part) + top * (long)sizeof(rank_t));
+}
+
+template <typename T>
+static void logprobs_run(RowsIn x, LogprobsOut o, LogprobsPlan p, long rows,
+                         long live, int cols, void* scratch, hipStream_t s) {
+  if (p.split > LP_PARTS) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_long_k<T>),
+                       dim3(row_grid(rows)), dim3(LP_THREADS), 0, s, x, o,
+                       rows, live, cols);
+    HIP_CHECK_LAST();
+    return;
+  }
+  const bool joined = p.split > 1;
+  rank_t* keys = joined ? (rank_t*)scratch : nullptr;
+  Part* parts =
+      joined ? (Part*)(keys + live * p.split * (long)o.top) : nullptr;
+  const long held = joined ? live : rows;
+#define NV_CASE(NV)                                                          \
+  case NV:                                                                   \
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_k<T, NV>),                   \
+                       parts_grid(p.split, held), dim3(LP_THREADS), 0, s, x, \
+                       o, held, live, cols, p.size, parts, keys);            \
+    break;
+  if (held) {
+    switch (p.nv) {
+      NV_CASE(1) NV_CASE(2) NV_CASE(4) NV_CASE(8) NV_CASE(16)
+    }
+    HIP_CHECK_LAST();
+  }
+#undef NV_CASE
+  if (!joined) return;
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_join_k<T>),
+                     dim3(row_grid(rows)), dim3(LP_THREADS),
+                     sizeof(rank_t) * p.split * o.top, s, x, o, parts, keys,
+                     rows, live, cols, p.split);
   HIP_CHECK_LAST();
 }
 
-void eval_distill_launch(int type, int err_type, RowsIn x, const int* idx, const float* z,
-                         RowsOut err, float* loss, const int* labels,
-                         int* n_err, int top, long rows, long live, int cols,
-                         float tau, hipStream_t s) {
+void token_logprobs_launch(int type, RowsIn x, const int* labels,
+                           float* logprob, float* entropy, int* top_idx,
+                           float* top_lp, int top, long rows, long live,
+                           int cols, void* scratch, hipStream_t s) {
+  if (rows == 0) return;
+  const LogprobsOut o{labels, logprob, entropy, top_idx, top_lp, top};
+  const LogprobsPlan p = logprobs_plan(type, live, cols);
+#define RUN(T) logprobs_run<T>(x, o, p, rows, live, cols, scratch, s)
+  ROW_TYPE_SWITCH(type, RUN)
+#undef RUN
+}
+
+void eval_distill_launch(int type, int err_type, RowsIn x, const int* idx,
+                         const float* z, RowsOut err, float* loss,
+                         const int* labels, int* n_err, int top, long rows,
+                         long live, int cols, float tau, hipStream_t s) {
   if (rows == 0) return;
 #define RUN2(T, O)                                                           \
   hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_k<T, O>), dim3(row_grid(rows)), \
