@@ -627,6 +627,7 @@ void token_logprobs(torch::Tensor x, Opt labels, Opt logprob, Opt entropy,
   const int type = row_type(op, x);
   const int64_t R = x.size(0), C = x.size(1);
   const int64_t live = live_rows(op, batch, R);
+  TORCH_CHECK(C <= (1 << 24), op, ": ", C, " classes of at most 2^24");
   TORCH_CHECK(logprob.has_value() == labels.has_value(), op,
               ": labels and logprob come together");
   TORCH_CHECK(top_idx.has_value() == top_lp.has_value(), op,

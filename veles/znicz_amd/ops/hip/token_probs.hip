@@ -244,16 +244,17 @@ template <typename T, int COUNT>
 __device__ __forceinline__ void add_packs(const Pack<T>* v, Sums& a, float c,
                                           float* high) {
   constexpr int N = Pack<T>::N;
-  float m = -INFINITY;
+  float m;
 #pragma unroll
   for (int i = 0; i < COUNT; ++i) {
     float e[N];
     v[i].get(e);
-    float h = e[0];
+    float h = max3(e[0], e[1], e[2]);
 #pragma unroll
-    for (int j = 1; j < N; ++j) h = fmaxf(h, e[j]);
+    for (int j = 3; j + 1 < N; j += 2) h = max3(h, e[j], e[j + 1]);
+    h = max3(h, e[N - 1], h);
     if (high) high[i] = h;
-    m = fmaxf(m, h);
+    m = i ? max3(m, h, m) : h;
   }
   a.raise(fmaxf(a.m, m), c);
 #pragma unroll
@@ -312,20 +313,25 @@ __device__ __forceinline__ void logprobs_padding(const LogprobsOut& o,
   }
 }
 
+// Logit of the class that is asked for: -inf if there is none, NaN for one
+// that does not exist; in thread 0.  (Read before the row is, as two loads
+// that wait for each other.)
 template <typename T>
+__device__ __forceinline__ float given_logit(const LogprobsOut& o, long row,
+                                             const T* x, int cols) {
+  if (threadIdx.x || !o.logprob) return 0.f;
+  const int l = o.labels[row];
+  return l >= cols ? NAN : l >= 0 ? (float)x[l] : -INFINITY;
+}
+
 __device__ __forceinline__ void logprobs_row(const LogprobsOut& o, long row,
-                                             const T* x, int cols,
-                                             const Row& r) {
+                                             float given, const Row& r) {
   if (threadIdx.x) return;
   if (o.entropy) o.entropy[row] = r.entropy;
   if (o.logprob) {
-    const int l = o.labels[row];
-    float v = 0.f;
-    if (l >= cols)
-      v = NAN;
-    else if (l >= 0)
-      v = r.bad ? NAN : r.none ? -INFINITY : ((float)x[l] - r.m) - r.ln;
-    o.logprob[row] = v;
+    const bool named = o.labels[row] >= 0;
+    const float v = given == -INFINITY ? given : (given - r.m) - r.ln;
+    o.logprob[row] = !named ? 0.f : r.bad ? NAN : v;
   }
 }
 
@@ -393,166 +399,310 @@ template <int THREADS>
 struct TopSpace {
   int high[THREADS];
   rank_t cand[LP_CAND];
-  int n, bound;
+  int n, bound, groups;
+  int list[LP_CAND];
   int tmp[THREADS / WAVE];
+
+  __device__ __forceinline__ void put(float x, float from, int j) {
+    if (x >= from) {
+      const int at = atomicAdd(&n, 1);
+      if (at < LP_CAND) cand[at] = rank_of(x, j);
+    }
+  }
 };
 
-// The `top` first classes of what the workgroup holds, as ranks in order in
-// cand[0..top); returns how many there are.  `high`: the largest value of
-// each pack of this thread.  Ends with all threads having their view of it.
-template <typename T, int THREADS, int NV>
-__device__ __forceinline__ int held_top(Held<T, THREADS, NV>& h, const T* x,
-                                        int n, int base, const float* high,
-                                        int top, TopSpace<THREADS>& sp,
-                                        rank_t* mine, int* place) {
-  constexpr int N = Pack<T>::N;
-  const int tid = threadIdx.x;
-  const int packs = h.whole(n);
-  if (tid < WAVE) {
+// The bound for all threads, from their largest values in sp.high
+template <int THREADS>
+__device__ __forceinline__ float share_bound(TopSpace<THREADS>& sp, int top) {
+  if (threadIdx.x < WAVE) {
     const int b = find_bound<THREADS>(sp.high, top);
-    if (tid == 0) {
+    if (threadIdx.x == 0) {
       sp.bound = b;
-      sp.n = 0;
+      sp.n = sp.groups = 0;
     }
   }
   __syncthreads();
-  const float bound = value_of(sp.bound);
-  auto put = [&](float x, int j) {
-    if (x >= bound) {
-      const int at = atomicAdd(&sp.n, 1);
-      if (at < LP_CAND) sp.cand[at] = rank_of(x, base + j);
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (i * THREADS >= packs) break;
-    if (high[i] >= bound) {
-      float e[N];
-      h.v[i].forget();
-      h.v[i].get(e);
-      const int p = (i * THREADS + tid) * N;
-#pragma unroll
-      for (int j = 0; j < N; ++j) put(e[j], p + j);
-    }
-  }
-  put(h.rest, h.rest_at(n));
-  __syncthreads();
-  int found = sp.n;
-  if (found > LP_CAND) {
-    // Too many reach the bound (one value many times): the top-th value
-    // itself, then among the classes that hold it the last that is needed,
-    // by halving; the part is read from the caches each time.
-    int lo = sp.bound, hi = 0x7f800000;
-    while (lo < hi) {
-      const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) / 2u);
-      int c = 0;
-      for (int j = tid; j < n; j += THREADS) c += order_of(x[j]) >= mid;
-      if (block_count<THREADS>(c, sp.tmp) >= top)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    int c = 0;
-    for (int j = tid; j < n; j += THREADS) c += order_of(x[j]) > lo;
-    const int need = top - block_count<THREADS>(c, sp.tmp);
-    int a = 0, b = n - 1;
-    while (a < b) {
-      const int mid = a + (b - a) / 2;
-      c = 0;
-      for (int j = tid; j <= mid; j += THREADS) c += order_of(x[j]) == lo;
-      if (block_count<THREADS>(c, sp.tmp) >= need)
-        b = mid;
-      else
-        a = mid + 1;
-    }
-    if (tid == 0) sp.n = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += THREADS) {
-      const int o = order_of(x[j]);
-      if (o > lo || (o == lo && j <= a))
-        sp.cand[atomicAdd(&sp.n, 1)] = rank_of(x[j], base + j);
-    }
-    __syncthreads();
-    found = sp.n;
-  }
-  // the place of each in the order is the number of those before it
-#pragma unroll
-  for (int i = 0; i * THREADS < LP_CAND; ++i) {
-    const int at = i * THREADS + tid;
-    mine[i] = at < found ? sp.cand[at] : 0;
-    int before = 0;
-    if (at < found)
-      for (int j = 0; j < found; ++j) before += sp.cand[j] > mine[i];
-    place[i] = before;
-  }
-  return found;
+  return value_of(sp.bound);
 }
 
-// One workgroup to a part of a row, which it holds in registers.  `parts`
-// null: it is the whole row, and the outputs are written; else its sums and
-// first classes, to be joined.
+// Too many classes reach the bound (one value many times): the top-th value
+// itself, then among the classes that hold it the last that is needed, by
+// halving; the part x[0..n) is read from the caches each time.
+template <typename T, int THREADS>
+__device__ __noinline__ void thin_out(const T* x, int n, int base, int top,
+                                      TopSpace<THREADS>& sp) {
+  const int tid = threadIdx.x;
+  int lo = sp.bound, hi = 0x7f800000;
+  while (lo < hi) {
+    const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) / 2u);
+    int c = 0;
+    for (int j = tid; j < n; j += THREADS) c += order_of(x[j]) >= mid;
+    if (block_count<THREADS>(c, sp.tmp) >= top)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  int c = 0;
+  for (int j = tid; j < n; j += THREADS) c += order_of(x[j]) > lo;
+  const int need = top - block_count<THREADS>(c, sp.tmp);
+  int a = 0, b = n - 1;
+  while (a < b) {
+    const int mid = a + (b - a) / 2;
+    c = 0;
+    for (int j = tid; j <= mid; j += THREADS) c += order_of(x[j]) == lo;
+    if (block_count<THREADS>(c, sp.tmp) >= need)
+      b = mid;
+    else
+      a = mid + 1;
+  }
+  if (tid == 0) sp.n = 0;
+  __syncthreads();
+  for (int j = tid; j < n; j += THREADS) {
+    const int o = order_of(x[j]);
+    if (o > lo || (o == lo && j <= a))
+      sp.cand[atomicAdd(&sp.n, 1)] = rank_of(x[j], base + j);
+  }
+  __syncthreads();
+}
+
+// what a workgroup's part of a row gives
+struct PartOut {
+  LogprobsOut o;
+  Part* parts;       // null: the part is the whole row
+  rank_t* keys;
+
+  __device__ __forceinline__ void put(long row, long item, int k, rank_t key,
+                                      const Row& r) const {
+    if (parts)
+      keys[item * o.top + k] = key;
+    else
+      logprobs_top(o, row, k, key, r);
+  }
+};
+
+// The `found` classes in sp.cand in their order: the place of each is the
+// number of those before it.
+template <int THREADS>
+__device__ __forceinline__ void put_top(const PartOut& p, long row, long item,
+                                        int found, const Row& r,
+                                        const TopSpace<THREADS>& sp) {
+  for (int i = threadIdx.x; i < found; i += THREADS) {
+    const rank_t mine = sp.cand[i];
+    int before = 0;
+    for (int j = 0; j < found; ++j) before += sp.cand[j] > mine;
+    if (before < p.o.top) p.put(row, item, before, mine, r);
+  }
+  for (int k = found + threadIdx.x; k < p.o.top; k += THREADS)
+    p.put(row, item, k, 0, r);
+}
+
+// Where u = C x - M does not do: the sums of the part x[0..n) once more
+template <typename T>
+__device__ __noinline__ Sums far_sums(const T* x, int n, float m, float c,
+                                      float* tmp) {
+  Sums a;
+  a.m = m;
+  a.um = 0.f;
+  a.s = a.w = 0.f;
+  for (int j = threadIdx.x; j < n; j += blockDim.x) {
+    const float u = ((float)x[j] - m) * c, e = pow2(u);
+    a.s += e;
+    a.w = fmaf(e, fmaxf(u, U_MIN), a.w);
+  }
+  __syncthreads();
+  a.s = block_sum(a.s, tmp);
+  a.w = block_sum(a.w, tmp);
+  return a;
+}
+
+// row, part and element range of this workgroup in a grid of parts x rows,
+// the rows in two dimensions
+struct Place {
+  long row, item;
+  int base, n;
+
+  __device__ __forceinline__ Place(int cols, int size) {
+    row = (long)blockIdx.z * gridDim.y + blockIdx.y;
+    item = row * gridDim.x + blockIdx.x;
+    base = blockIdx.x * size;
+    n = min(size, cols - base);
+  }
+};
+
+// One workgroup to a part of a row, which it holds in registers
 template <typename T, int NV>
-__global__ __launch_bounds__(LP_THREADS) void logprobs_k(
-    RowsIn x_, LogprobsOut o, long rows, long live, int cols, int size,
-    Part* __restrict__ parts, rank_t* __restrict__ keys) {
+__global__ __launch_bounds__(LP_THREADS) void logprobs_held_k(
+    RowsIn x_, PartOut p, long rows, long live, int cols, int size) {
   __shared__ TopSpace<LP_THREADS> sp;
   __shared__ Sums tmp[LP_THREADS / WAVE];
+  constexpr int N = Pack<T>::N;
   const int tid = threadIdx.x;
-  // (a grid of parts x rows, the rows in two dimensions)
-  const long row = (long)blockIdx.z * gridDim.y + blockIdx.y;
-  if (row >= rows) return;
-  const int seg = blockIdx.x;
-  const long item = row * gridDim.x + seg;
-  if (row >= live) {
-    logprobs_padding(o, row);
+  const Place at(cols, size);
+  if (at.row >= rows) return;
+  if (at.row >= live) {
+    logprobs_padding(p.o, at.row);
     return;
   }
-  const T* x = (const T*)x_.p + row * x_.stride;
-  const int base = seg * size;
-  const int n = min(size, cols - base);
+  const T* row = (const T*)x_.p + at.row * x_.stride;
+  const T* x = row + at.base;
+  const float given = p.parts ? 0.f : given_logit(p.o, at.row, row, cols);
   Held<T, LP_THREADS, NV> h;
-  h.load(x + base, n);
+  h.load(x, at.n);
   float high[NV];
-  Sums a = held_sums(h, n, LOG2E, high);
+  Sums a = held_sums(h, at.n, LOG2E, high);
   sp.high[tid] = order_of(a.m);
   a = join_block<LP_THREADS>(a, LOG2E, tmp);
-  if (is_far(a.m, LOG2E)) {
-    float s = 0.f, w = 0.f;
-    for (int j = tid; j < n; j += LP_THREADS) {
-      const float u = ((float)x[base + j] - a.m) * LOG2E, e = pow2(u);
-      s += e;
-      w = fmaf(e, fmaxf(u, U_MIN), w);
-    }
-    __syncthreads();
-    a.s = block_sum(s, (float*)tmp);
-    a.w = block_sum(w, (float*)tmp);
-  }
+  if (is_far(a.m, LOG2E)) a = far_sums(x, at.n, a.m, LOG2E, (float*)tmp);
   Row r;
   r.finish(a, LOG2E);
-  if (parts) {
-    if (tid == 0) parts[item] = part_of(a, LOG2E, 0);
-  } else {
-    logprobs_row(o, row, x, cols, r);
-  }
-  if (!o.top) return;
-  rank_t mine[LP_CAND / LP_THREADS];
-  int place[LP_CAND / LP_THREADS], found = 0;
-  if (!r.bad && !r.none)
-    found = held_top(h, x + base, n, base, high, o.top, sp, mine, place);
+  if (!p.parts)
+    logprobs_row(p.o, at.row, given, r);
+  else if (tid == 0)
+    p.parts[at.item] = part_of(a, LOG2E, 0);
+  if (!p.o.top) return;
+  int found = 0;
+  if (!r.bad && !r.none) {
+    const float bound = share_bound(sp, p.o.top);
+    const int packs = h.whole(at.n);
 #pragma unroll
-  for (int i = 0; i < LP_CAND / LP_THREADS; ++i)
-    if (i * LP_THREADS + tid < found && place[i] < o.top) {
-      if (parts)
-        keys[item * o.top + place[i]] = mine[i];
-      else
-        logprobs_top(o, row, place[i], mine[i], r);
+    for (int i = 0; i < NV; ++i) {
+      if (i * LP_THREADS >= packs) break;
+      if (high[i] >= bound) {
+        float e[N];
+        h.v[i].forget();
+        h.v[i].get(e);
+        const int j0 = at.base + (i * LP_THREADS + tid) * N;
+#pragma unroll
+        for (int j = 0; j < N; ++j) sp.put(e[j], bound, j0 + j);
+      }
     }
-  for (int k = found + tid; k < o.top; k += LP_THREADS) {
-    if (parts)
-      keys[item * o.top + k] = 0;
-    else
-      logprobs_top(o, row, k, 0, r);
+    sp.put(h.rest, bound, at.base + h.rest_at(at.n));
+    __syncthreads();
+    if (sp.n > LP_CAND)
+      thin_out<T, LP_THREADS>(x, at.n, at.base, p.o.top, sp);
+    found = sp.n;
   }
+  put_top(p, at.row, at.item, found, r, sp);
+}
+
+// largest value of the eight lanes' own, for four values; in all lanes
+__device__ __forceinline__ void max_of_eight_lanes(float* h) {
+  // (two wait states between a write and its use by another lane)
+  asm volatile("s_nop 1\n\t"
+      "v_max_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %1, %1, %1 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %2, %2, %2 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %3, %3, %3 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %1, %1, %1 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %2, %2, %2 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %3, %3, %3 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %1, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %2, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+      "v_max_f32_dpp %3, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xf"
+      : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]));
+}
+
+// One workgroup to a part of a row that streams past it, four packs of a
+// thread at a time.  The largest value of each eight packs (128 bytes) stays
+// in LDS; for the alternatives those are read again that reach the bound.
+#define GROUP 8
+template <typename T, bool TOP>
+__global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
+    RowsIn x_, PartOut p, long rows, long live, int cols, int size) {
+  __shared__ TopSpace<LP_THREADS> sp;
+  __shared__ Sums tmp[LP_THREADS / WAVE];
+  extern __shared__ float groups[];
+  constexpr int N = Pack<T>::N;
+  constexpr int U = 4, STEP = U * LP_THREADS;
+  const int tid = threadIdx.x;
+  const Place at(cols, size);
+  if (at.row >= rows) return;
+  if (at.row >= live) {
+    logprobs_padding(p.o, at.row);
+    return;
+  }
+  const T* row = (const T*)x_.p + at.row * x_.stride;
+  const T* x = row + at.base;
+  const float given = p.parts ? 0.f : given_logit(p.o, at.row, row, cols);
+  const int packs = at.n / N;
+  const int rest_at = packs * N + tid;
+  const float rest = rest_at < at.n ? (float)x[rest_at] : -INFINITY;
+  Sums a;
+  a.clear();
+  a.raise(rest, LOG2E);
+  a.add(rest, LOG2E);
+  for (int b = 0; b < packs; b += STEP) {
+    Pack<T> v[U];
+    if (b + STEP <= packs) {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        v[i].load_once(x + (long)(b + i * LP_THREADS) * N + tid * N);
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        v[i].fill(-INFINITY);
+        if (b + i * LP_THREADS + tid < packs)
+          v[i].load_once(x + (long)(b + i * LP_THREADS) * N + tid * N);
+      }
+    }
+    float high[U];
+    add_packs<T, U>(v, a, LOG2E, high);
+    if (TOP) {
+      max_of_eight_lanes(high);
+      // lane i of each eight has that of pack row i
+      const int i = tid % GROUP;
+      const float h = i == 0 ? high[0] : i == 1 ? high[1]
+                    : i == 2 ? high[2] : high[3];
+      const int g = (b + i * LP_THREADS + tid) / GROUP;
+      if (i < U && g * GROUP < packs) groups[g] = h;
+    }
+  }
+  a = join_block<LP_THREADS>(a, LOG2E, tmp);
+  if (is_far(a.m, LOG2E)) a = far_sums(x, at.n, a.m, LOG2E, (float*)tmp);
+  Row r;
+  r.finish(a, LOG2E);
+  if (!p.parts)
+    logprobs_row(p.o, at.row, given, r);
+  else if (tid == 0)
+    p.parts[at.item] = part_of(a, LOG2E, 0);
+  if (!TOP) return;
+  int found = 0;
+  if (!r.bad && !r.none) {
+    const int n = (packs + GROUP - 1) / GROUP;
+    float h = rest;
+    for (int g = tid; g < n; g += LP_THREADS) h = fmaxf(h, groups[g]);
+    sp.high[tid] = order_of(h);
+    __syncthreads();
+    const float bound = share_bound(sp, p.o.top);
+    if (h >= bound)
+      for (int g = tid; g < n; g += LP_THREADS)
+        if (groups[g] >= bound) {
+          const int k = atomicAdd(&sp.groups, 1);
+          if (k < LP_CAND) sp.list[k] = g;
+        }
+    sp.put(rest, bound, at.base + rest_at);
+    __syncthreads();
+    const int m = min(sp.groups, LP_CAND);
+    for (int k = tid / GROUP; k < m; k += LP_THREADS / GROUP) {
+      const int q = sp.list[k] * GROUP + tid % GROUP;
+      if (q < packs) {
+        Pack<T> v;
+        float e[N];
+        v.load(x + (long)q * N);
+        v.get(e);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          sp.put(e[j], bound, at.base + q * N + j);
+      }
+    }
+    __syncthreads();
+    if (sp.n > LP_CAND || sp.groups > LP_CAND)
+      thin_out<T, LP_THREADS>(x, at.n, at.base, p.o.top, sp);
+    found = sp.n;
+  }
+  put_top(p, at.row, at.item, found, r, sp);
 }
 
 // A row's parts joined.  Their classes are in order, so that the place of
@@ -572,9 +722,10 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_k(
     const int all = split * o.top;
     for (int i = threadIdx.x; i < all; i += LP_THREADS)
       list[i] = keys[row * all + i];
+    const float given = given_logit(o, row, x, cols);
     int first;
     const Row r = join_parts(parts + row * split, split, LOG2E, &first);
-    logprobs_row(o, row, x, cols, r);
+    logprobs_row(o, row, given, r);
     __syncthreads();
     if (r.bad || r.none) {
       for (int k = threadIdx.x; k < o.top; k += LP_THREADS)
@@ -602,65 +753,6 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_k(
       }
     }
     __syncthreads();
-  }
-}
-
-// Rows of more classes than parts of registers are joined for: one
-// workgroup to a row, which is read again for each alternative.
-template <typename T>
-__global__ __launch_bounds__(LP_THREADS) void logprobs_long_k(
-    RowsIn x_, LogprobsOut o, long rows, long live, int cols) {
-  __shared__ Sums tmp[LP_THREADS / WAVE];
-  __shared__ rank_t ktmp[LP_THREADS / WAVE];
-  const int tid = threadIdx.x;
-  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
-    if (row >= live) {
-      logprobs_padding(o, row);
-      continue;
-    }
-    const T* x = (const T*)x_.p + row * x_.stride;
-    float m = -INFINITY;
-    for (int j = tid; j < cols; j += LP_THREADS) m = fmaxf(m, (float)x[j]);
-    m = block_max(m, (float*)tmp);
-    const bool far = is_far(m, LOG2E);
-    Sums a;
-    a.clear();
-    a.m = m;
-    a.um = fmaxf(m * LOG2E, M_MIN);
-    for (int j = tid; j < cols; j += LP_THREADS) {
-      const float v = (float)x[j];
-      const float u = far ? (v - m) * LOG2E : fmaf(v, LOG2E, -a.um);
-      const float e = pow2(u);
-      a.s += e;
-      a.w = fmaf(e, fmaxf(u, U_MIN), a.w);
-    }
-    a.s = block_sum(a.s, (float*)tmp);
-    a.w = block_sum(a.w, (float*)tmp);
-    Row r;
-    r.finish(a, LOG2E);
-    logprobs_row(o, row, x, cols, r);
-    rank_t last = ~0ull;
-    for (int k = 0; k < o.top; ++k) {
-      rank_t best = 0;
-      if (!r.bad && !r.none && last)
-        for (int j = tid; j < cols; j += LP_THREADS) {
-          const float v = (float)x[j];
-          const rank_t key = v == -INFINITY ? 0 : rank_of(v, j);
-          if (key < last && key > best) best = key;
-        }
-#pragma unroll
-      for (int off = 32; off; off >>= 1) {
-        const rank_t other = __shfl_xor(best, off);
-        best = other > best ? other : best;
-      }
-      if ((tid & (WAVE - 1)) == 0) ktmp[tid / WAVE] = best;
-      __syncthreads();
-      for (int i = 0; i < LP_THREADS / WAVE; ++i)
-        best = ktmp[i] > best ? ktmp[i] : best;
-      __syncthreads();
-      if (tid == 0) logprobs_top(o, row, k, best, r);
-      last = best;
-    }
   }
 }
 
@@ -795,17 +887,20 @@ static dim3 parts_grid(int split, long rows) {
   return dim3((unsigned)split, (unsigned)y, (unsigned)((rows + y - 1) / y));
 }
 
-// parts of a row that are joined at most, and ranks of them in LDS
+// parts of a row that are joined at most, and groups that a part may have
 #define LP_PARTS 64
+#define LP_GROUPS 16384
 
-// How a call is laid out: packs of a thread, parts of a row
+// How a call is laid out: parts of a row, elements of a part, and packs of
+// a thread where they are held (0: they stream past)
 struct LogprobsPlan {
-  int nv, split, size;
+  int split, size, nv;
 };
 
 static LogprobsPlan logprobs_plan(int type, long rows, int cols) {
   const int n = type == ROW_F32 ? 4 : 8;
-  const int most = LP_THREADS * 16 * n;
+  const long held = LP_THREADS * 16 * n;
+  const long most = (long)LP_GROUPS * GROUP * n;
   long split = (cols + most - 1) / most;
   // few rows: parts of at least 4 packs a thread, up to two workgroups for
   // each compute unit
@@ -813,58 +908,67 @@ static LogprobsPlan logprobs_plan(int type, long rows, int cols) {
   while (split < LP_PARTS && rows * split < 512 &&
          cols / (split + 1) >= least)
     ++split;
-  LogprobsPlan p;
-  p.split = (int)split;
   // whole packs to a part
   long size = (cols + split - 1) / split;
   size = (size + n - 1) / n * n;
+  LogprobsPlan p;
   p.size = (int)size;
   p.split = (int)((cols + size - 1) / size);
-  p.nv = 1;
-  while ((long)LP_THREADS * p.nv * n < size && p.nv < 16) p.nv *= 2;
+  p.nv = 0;
+  if (size <= held) {
+    p.nv = 1;
+    while ((long)LP_THREADS * p.nv * n < size) p.nv *= 2;
+  }
   return p;
 }
 
 // bytes that token_logprobs_launch needs at `scratch`
 long token_logprobs_scratch(int type, long live, int cols, int top) {
   const LogprobsPlan p = logprobs_plan(type, live, cols);
-  if (p.split == 1 || p.split > LP_PARTS) return 0;
+  if (p.split == 1) return 0;
   return live * p.split * ((long)sizeof(Part) + top * (long)sizeof(rank_t));
 }
 
 template <typename T>
-static void logprobs_run(RowsIn x, LogprobsOut o, LogprobsPlan p, long rows,
+static void logprobs_run(RowsIn x, LogprobsOut o, LogprobsPlan l, long rows,
                          long live, int cols, void* scratch, hipStream_t s) {
-  if (p.split > LP_PARTS) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_long_k<T>),
-                       dim3(row_grid(rows)), dim3(LP_THREADS), 0, s, x, o,
-                       rows, live, cols);
-    HIP_CHECK_LAST();
-    return;
+  const bool joined = l.split > 1;
+  PartOut p{o, nullptr, nullptr};
+  if (joined) {
+    p.keys = (rank_t*)scratch;
+    p.parts = (Part*)(p.keys + live * l.split * (long)o.top);
   }
-  const bool joined = p.split > 1;
-  rank_t* keys = joined ? (rank_t*)scratch : nullptr;
-  Part* parts =
-      joined ? (Part*)(keys + live * p.split * (long)o.top) : nullptr;
-  const long held = joined ? live : rows;
-#define NV_CASE(NV)                                                          \
+  const long some = joined ? live : rows;
+#define HELD(NV)                                                             \
   case NV:                                                                   \
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_k<T, NV>),                   \
-                       parts_grid(p.split, held), dim3(LP_THREADS), 0, s, x, \
-                       o, held, live, cols, p.size, parts, keys);            \
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_held_k<T, NV>),              \
+                       parts_grid(l.split, some), dim3(LP_THREADS), 0, s, x, \
+                       p, some, live, cols, l.size);                         \
     break;
-  if (held) {
-    switch (p.nv) {
-      NV_CASE(1) NV_CASE(2) NV_CASE(4) NV_CASE(8) NV_CASE(16)
+#define STREAM(TOP)                                                          \
+  hipLaunchKernelGGL(                                                        \
+      HIP_KERNEL_NAME(logprobs_stream_k<T, TOP>), parts_grid(l.split, some), \
+      dim3(LP_THREADS),                                                      \
+      TOP ? (l.size / Pack<T>::N + GROUP - 1) / GROUP * sizeof(float) : 0,   \
+      s, x, p, some, live, cols, l.size)
+  if (some) {
+    switch (l.nv) {
+      HELD(1) HELD(2) HELD(4) HELD(8) HELD(16)
+      default:
+        if (o.top)
+          STREAM(true);
+        else
+          STREAM(false);
     }
     HIP_CHECK_LAST();
   }
-#undef NV_CASE
+#undef HELD
+#undef STREAM
   if (!joined) return;
   hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_join_k<T>),
                      dim3(row_grid(rows)), dim3(LP_THREADS),
-                     sizeof(rank_t) * p.split * o.top, s, x, o, parts, keys,
-                     rows, live, cols, p.split);
+                     sizeof(rank_t) * l.split * o.top, s, x, o, p.parts,
+                     p.keys, rows, live, cols, l.split);
   HIP_CHECK_LAST();
 }
 
