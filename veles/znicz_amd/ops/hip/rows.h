@@ -12,16 +12,43 @@ typedef _Float16 f16_t;
 template <typename T>
 __device__ __forceinline__ T from_f(float f) { return (T)f; }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
-  return v;
+// Over the 64 lanes of a wave, all of them at work; the result in every lane.
+// Sixteen lanes are joined through the operands of the instructions
+// themselves (a shuffle goes through LDS, at ten times the delay).
+template <int CTRL, typename V>
+__device__ __forceinline__ V other_lane(V v) {
+  return __builtin_bit_cast(
+      V, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf,
+                                  true));
 }
-
+template <typename V>
+__device__ __forceinline__ V lane_of(V v, int lane) {
+  return __builtin_bit_cast(
+      V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+template <typename V, typename F>
+__device__ __forceinline__ V wave_join(V v, F f) {
+  v = f(v, other_lane<0xb1>(v));     // lanes 1 0 3 2
+  v = f(v, other_lane<0x4e>(v));     // 2 3 0 1
+  v = f(v, other_lane<0x141>(v));    // 7 ... 0
+  v = f(v, other_lane<0x140>(v));    // 15 ... 0
+  return f(f(lane_of(v, 0), lane_of(v, 16)),
+           f(lane_of(v, 32), lane_of(v, 48)));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return wave_join(v, [](float a, float b) { return a + b; });
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
-  return v;
+  return wave_join(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ int wave_max(int v) {
+  return wave_join(v, [](int a, int b) { return max(a, b); });
+}
+__device__ __forceinline__ int wave_min(int v) {
+  return wave_join(v, [](int a, int b) { return min(a, b); });
+}
+__device__ __forceinline__ int wave_sum(int v) {
+  return wave_join(v, [](int a, int b) { return a + b; });
 }
 
 // Sum over the workgroup, in every thread.  `tmp`: one float for each wave,

@@ -60,8 +60,21 @@ __device__ __forceinline__ rank_t rank_of(float x, int j) {
 __device__ __forceinline__ float rank_value(rank_t k) {
   return value_of((int)((unsigned)(k >> 32) ^ 0x80000000u));
 }
+// (of key 0: below that of every value)
+__device__ __forceinline__ int rank_order(rank_t k) {
+  return (int)((unsigned)(k >> 32) ^ 0x80000000u);
+}
 __device__ __forceinline__ int rank_class(rank_t k) {
   return 0x7fffffff - (int)(unsigned)k;
+}
+
+// how many of the list are before one
+__device__ __forceinline__ int ranks_before(const rank_t* list, int n,
+                                            rank_t key) {
+  int before = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; ++j) before += list[j] > key;
+  return before;
 }
 
 // ---------------------------------------------------------------------------
@@ -170,30 +183,26 @@ __device__ __forceinline__ Part part_of(const Sums& a, float c, int first) {
   return Part{a.m, f * a.s, f * fmaf(-d, a.s, a.w), first};
 }
 
-// n parts of a row joined, by every thread for itself
+// Up to 64 parts of a row joined, by every wave for itself: lane i has the
+// i-th.
 __device__ __forceinline__ Row join_parts(const Part* p, int n, float c,
                                           int* first) {
-  float m = -INFINITY;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, p[i].m);
-  float s = 0.f, w = 0.f;
-  int at = 0x7fffffff;
-  for (int i = 0; i < n; ++i) {
-    // (an empty part beside an empty row: no difference of infinities)
-    const float by = p[i].m == m ? 0.f : fmaxf((p[i].m - m) * c, M_MIN);
-    const float f = pow2(by);
-    s = fmaf(f, p[i].s, s);
-    w = fmaf(f, fmaf(by, p[i].s, p[i].w), w);
-    if (p[i].m == m) at = min(at, p[i].first);
-  }
-  Sums a;
-  a.m = m;
-  a.um = fmaxf(m * c, M_MIN);
-  a.s = s;
-  a.w = w;
+  const int lane = threadIdx.x & (WAVE - 1);
+  Part a{-INFINITY, 0.f, 0.f, 0x7fffffff};
+  if (lane < n) a = p[lane];
+  const float m = wave_max(a.m);
+  // (an empty part beside an empty row: no difference of infinities)
+  const float by = a.m == m ? 0.f : fmaxf((a.m - m) * c, M_MIN);
+  const float f = pow2(by);
+  Sums t;
+  t.m = m;
+  t.um = fmaxf(m * c, M_MIN);
+  t.s = wave_sum(f * a.s);
+  t.w = wave_sum(f * fmaf(by, a.s, a.w));
+  *first = wave_min(a.m == m ? a.first : 0x7fffffff);
   Row r;
-  r.finish(a, c);
-  r.ln = log2_of(s) * LN2;               // (the parts are to the exact C m)
-  *first = at;
+  r.finish(t, c);
+  r.ln = log2_of(t.s) * LN2;             // (the parts are to the exact C m)
   return r;
 }
 
@@ -201,38 +210,45 @@ __device__ __forceinline__ Row join_parts(const Part* p, int n, float c,
 // a row, or a part of it, in the registers of a workgroup
 // ---------------------------------------------------------------------------
 
-// Thread t holds packs t, t + THREADS, ... and one of the last elements that
-// make no whole pack.  Places without an element hold minus infinity.
+// A row's elements: up to N - 1 before the first multiple of 16 bytes (loads
+// off such a multiple are slower: 4096 x 50001 bf16 in 95 us, x 50000 in 79),
+// whole packs, and up to N - 1 behind them.  The single ones are one each for
+// the first 2 N threads.
+template <typename T>
+struct Cut {
+  static constexpr int N = Pack<T>::N;
+  int head, packs, single;     // single: this thread's, or -1
+
+  __device__ __forceinline__ Cut(const T* x, int n) {
+    head = (int)((16 - ((unsigned long long)x & 15)) & 15) / (int)sizeof(T);
+    head = min(head, n);
+    packs = (n - head) / N;
+    const int tail = head + packs * N, t = threadIdx.x;
+    single = t < head ? t : t >= N && tail + t - N < n ? tail + t - N : -1;
+  }
+  __device__ __forceinline__ float load_single(const T* x) const {
+    return single >= 0 ? (float)x[single] : -INFINITY;
+  }
+};
+
+// Thread t holds packs t, t + THREADS, ... and one of the single elements.
+// Places without an element hold minus infinity.
 template <typename T, int THREADS, int NV>
 struct Held {
   static constexpr int N = Pack<T>::N;
-  static constexpr int MOST = THREADS * NV * N;
   Pack<T> v[NV];
   float rest;
 
-  __device__ __forceinline__ static int whole(int n) {
-    const int packs = n / N;
-    return packs < THREADS * NV ? packs : THREADS * NV;
-  }
-  // place of the element `rest`; those beyond it (a row longer than MOST)
-  // are left to the caller
-  __device__ __forceinline__ static int rest_at(int n) {
-    return n / N * N + threadIdx.x;
-  }
-
-  __device__ __forceinline__ void load(const T* x, int n) {
-    const int packs = whole(n);
+  __device__ __forceinline__ void load(const T* x, const Cut<T>& cut) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int p = i * THREADS + threadIdx.x;
       v[i].fill(-INFINITY);
       // (one offset for all, from bases that are the same for a wave)
-      if (p < packs) v[i].load(x + i * THREADS * N + threadIdx.x * N);
+      if (i * THREADS + (int)threadIdx.x < cut.packs)
+        v[i].load_once(x + cut.head + i * THREADS * N + threadIdx.x * N);
     }
-    const int j = rest_at(n);
-    rest = j < n ? (float)x[j] : -INFINITY;
+    rest = cut.load_single(x);
   }
-
 };
 
 // Packs are summed CHUNK at a time, relative to the thread's largest so far:
@@ -268,9 +284,8 @@ __device__ __forceinline__ void add_packs(const Pack<T>* v, Sums& a, float c,
 
 template <typename T, int THREADS, int NV>
 __device__ __forceinline__ Sums held_sums(const Held<T, THREADS, NV>& h,
-                                          int n, float c, float* high) {
+                                          int packs, float c, float* high) {
   constexpr int STEP = NV < CHUNK ? NV : CHUNK;
-  const int packs = h.whole(n);
   Sums a;
   a.clear();
 #pragma unroll
@@ -347,8 +362,7 @@ __device__ __forceinline__ void logprobs_top(const LogprobsOut& o, long row,
 template <int THREADS>
 __device__ __forceinline__ int block_count(int n, int* tmp) {
   constexpr int WAVES = THREADS / WAVE;
-#pragma unroll
-  for (int off = 32; off; off >>= 1) n += __shfl_xor(n, off);
+  n = wave_sum(n);
   __syncthreads();
   if ((threadIdx.x & (WAVE - 1)) == 0) tmp[threadIdx.x / WAVE] = n;
   __syncthreads();
@@ -371,8 +385,7 @@ __device__ __forceinline__ int find_bound(const int* high, int top) {
   int hi = v[0];
 #pragma unroll
   for (int i = 1; i < PER; ++i) hi = max(hi, v[i]);
-#pragma unroll
-  for (int off = 32; off; off >>= 1) hi = max(hi, __shfl_xor(hi, off));
+  hi = wave_max(hi);
   int lo = ORDER_NONE + 1;
   auto reach = [&](int b) {
     int n = 0;
@@ -488,8 +501,7 @@ __device__ __forceinline__ void put_top(const PartOut& p, long row, long item,
                                         const TopSpace<THREADS>& sp) {
   for (int i = threadIdx.x; i < found; i += THREADS) {
     const rank_t mine = sp.cand[i];
-    int before = 0;
-    for (int j = 0; j < found; ++j) before += sp.cand[j] > mine;
+    const int before = ranks_before(sp.cand, found, mine);
     if (before < p.o.top) p.put(row, item, before, mine, r);
   }
   for (int k = found + threadIdx.x; k < p.o.top; k += THREADS)
@@ -546,10 +558,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_held_k(
   const T* row = (const T*)x_.p + at.row * x_.stride;
   const T* x = row + at.base;
   const float given = p.parts ? 0.f : given_logit(p.o, at.row, row, cols);
+  const Cut<T> cut(x, at.n);
   Held<T, LP_THREADS, NV> h;
-  h.load(x, at.n);
+  h.load(x, cut);
   float high[NV];
-  Sums a = held_sums(h, at.n, LOG2E, high);
+  Sums a = held_sums(h, cut.packs, LOG2E, high);
   sp.high[tid] = order_of(a.m);
   a = join_block<LP_THREADS>(a, LOG2E, tmp);
   if (is_far(a.m, LOG2E)) a = far_sums(x, at.n, a.m, LOG2E, (float*)tmp);
@@ -563,20 +576,19 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_held_k(
   int found = 0;
   if (!r.bad && !r.none) {
     const float bound = share_bound(sp, p.o.top);
-    const int packs = h.whole(at.n);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (i * LP_THREADS >= packs) break;
+      if (i * LP_THREADS >= cut.packs) break;
       if (high[i] >= bound) {
         float e[N];
         h.v[i].forget();
         h.v[i].get(e);
-        const int j0 = at.base + (i * LP_THREADS + tid) * N;
+        const int j0 = at.base + cut.head + (i * LP_THREADS + tid) * N;
 #pragma unroll
         for (int j = 0; j < N; ++j) sp.put(e[j], bound, j0 + j);
       }
     }
-    sp.put(h.rest, bound, at.base + h.rest_at(at.n));
+    sp.put(h.rest, bound, at.base + cut.single);
     __syncthreads();
     if (sp.n > LP_CAND)
       thin_out<T, LP_THREADS>(x, at.n, at.base, p.o.top, sp);
@@ -626,9 +638,10 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
   const T* row = (const T*)x_.p + at.row * x_.stride;
   const T* x = row + at.base;
   const float given = p.parts ? 0.f : given_logit(p.o, at.row, row, cols);
-  const int packs = at.n / N;
-  const int rest_at = packs * N + tid;
-  const float rest = rest_at < at.n ? (float)x[rest_at] : -INFINITY;
+  const Cut<T> cut(x, at.n);
+  const int packs = cut.packs;
+  const float rest = cut.load_single(x);
+  const T* body = x + cut.head;
   Sums a;
   a.clear();
   a.raise(rest, LOG2E);
@@ -638,13 +651,13 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
     if (b + STEP <= packs) {
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        v[i].load_once(x + (long)(b + i * LP_THREADS) * N + tid * N);
+        v[i].load_once(body + (long)(b + i * LP_THREADS) * N + tid * N);
     } else {
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         v[i].fill(-INFINITY);
         if (b + i * LP_THREADS + tid < packs)
-          v[i].load_once(x + (long)(b + i * LP_THREADS) * N + tid * N);
+          v[i].load_once(body + (long)(b + i * LP_THREADS) * N + tid * N);
       }
     }
     float high[U];
@@ -682,7 +695,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
           const int k = atomicAdd(&sp.groups, 1);
           if (k < LP_CAND) sp.list[k] = g;
         }
-    sp.put(rest, bound, at.base + rest_at);
+    sp.put(rest, bound, at.base + cut.single);
     __syncthreads();
     const int m = min(sp.groups, LP_CAND);
     for (int k = tid / GROUP; k < m; k += LP_THREADS / GROUP) {
@@ -690,11 +703,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
       if (q < packs) {
         Pack<T> v;
         float e[N];
-        v.load(x + (long)q * N);
+        v.load(body + (long)q * N);
         v.get(e);
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          sp.put(e[j], bound, at.base + q * N + j);
+          sp.put(e[j], bound, at.base + cut.head + q * N + j);
       }
     }
     __syncthreads();
@@ -705,14 +718,18 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
   put_top(p, at.row, at.item, found, r, sp);
 }
 
-// A row's parts joined.  Their classes are in order, so that the place of
-// one among all is found by halving each part's list.
+// A row's parts joined.  Each part's list is in order, so that the first few
+// of all lists, one to a thread, have a bound as the threads' largest values
+// have within a part.
 template <typename T>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_join_k(
     RowsIn x_, LogprobsOut o, const Part* __restrict__ parts,
     const rank_t* __restrict__ keys, long rows, long live, int cols,
     int split) {
   extern __shared__ rank_t list[];
+  __shared__ int high[LP_THREADS];
+  __shared__ int count, bound;
+  const int tid = threadIdx.x;
   for (long row = blockIdx.x; row < rows; row += gridDim.x) {
     if (row >= live) {
       logprobs_padding(o, row);
@@ -720,38 +737,39 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_k(
     }
     const T* x = (const T*)x_.p + row * x_.stride;
     const int all = split * o.top;
-    for (int i = threadIdx.x; i < all; i += LP_THREADS)
-      list[i] = keys[row * all + i];
+    const rank_t* mine = keys + row * all;
+    const int place = tid / split;
+    rank_t k = 0;
+    if (place < o.top && place < LP_THREADS / split)
+      k = mine[tid % split * o.top + place];
     const float given = given_logit(o, row, x, cols);
     int first;
     const Row r = join_parts(parts + row * split, split, LOG2E, &first);
     logprobs_row(o, row, given, r);
+    if (!o.top) continue;
+    high[tid] = rank_order(k);
     __syncthreads();
-    if (r.bad || r.none) {
-      for (int k = threadIdx.x; k < o.top; k += LP_THREADS)
-        logprobs_top(o, row, k, 0, r);
-    } else {
-      for (int i = threadIdx.x; i < all; i += LP_THREADS) {
-        const rank_t key = list[i];
-        const int own = i / o.top;
-        // empty places come last, in the order of the list
-        int before = i - own * o.top;
-        for (int p = 0; p < split && before < o.top; ++p) {
-          if (p == own) continue;
-          int lo = 0, hi = o.top;        // the first that is not before it
-          while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            const rank_t other = list[p * o.top + mid];
-            if (other > key || (other == key && p < own))
-              lo = mid + 1;
-            else
-              hi = mid;
-          }
-          before += lo;
-        }
-        if (before < o.top) logprobs_top(o, row, before, key, r);
+    if (tid < WAVE) {
+      const int b = find_bound<LP_THREADS>(high, o.top);
+      if (tid == 0) {
+        bound = b;
+        count = 0;
       }
     }
+    __syncthreads();
+    if (!r.bad && !r.none)
+      for (int i = tid; i < all; i += LP_THREADS) {
+        const rank_t k = mine[i];
+        if (rank_order(k) >= bound) list[atomicAdd(&count, 1)] = k;
+      }
+    __syncthreads();
+    const int found = count;
+    for (int i = tid; i < found; i += LP_THREADS) {
+      const int before = ranks_before(list, found, list[i]);
+      if (before < o.top) logprobs_top(o, row, before, list[i], r);
+    }
+    for (int k = found + tid; k < o.top; k += LP_THREADS)
+      logprobs_top(o, row, k, 0, r);
     __syncthreads();
   }
 }
@@ -890,6 +908,12 @@ static dim3 parts_grid(int split, long rows) {
 // parts of a row that are joined at most, and groups that a part may have
 #define LP_PARTS 64
 #define LP_GROUPS 16384
+// Few rows are cut until there are two workgroups for each compute unit, but
+// into parts of 4 packs a thread at least.  One row of 131072 bf16: 11.0 us
+// with 4 packs, 11.0 with 2; 600 rows: 38 us with two workgroups, 41 with
+// four, 39 with eight (the parts' own ends and their joining weigh more).
+#define LP_LEAST 4
+#define LP_BLOCKS 512
 
 // How a call is laid out: parts of a row, elements of a part, and packs of
 // a thread where they are held (0: they stream past)
@@ -902,10 +926,8 @@ static LogprobsPlan logprobs_plan(int type, long rows, int cols) {
   const long held = LP_THREADS * 16 * n;
   const long most = (long)LP_GROUPS * GROUP * n;
   long split = (cols + most - 1) / most;
-  // few rows: parts of at least 4 packs a thread, up to two workgroups for
-  // each compute unit
-  const long least = LP_THREADS * 4 * n;
-  while (split < LP_PARTS && rows * split < 512 &&
+  const long least = LP_THREADS * LP_LEAST * n;
+  while (split < LP_PARTS && rows * split < LP_BLOCKS &&
          cols / (split + 1) >= least)
     ++split;
   // whole packs to a part
