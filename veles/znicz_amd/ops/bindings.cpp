@@ -95,7 +95,8 @@ void token_logprobs_launch(int, RowsIn, const int*, float*, float*, int*,
                            hipStream_t);
 void eval_distill_launch(int, int, RowsIn, const int*, const float*, RowsOut,
                          float*, const int*, int*, int, long, long, int,
-                         float, hipStream_t);
+                         float, void*, hipStream_t);
+long eval_distill_scratch(int, long, int, int);
 
 namespace {
 
@@ -696,9 +697,16 @@ void eval_distill(torch::Tensor x, torch::Tensor idx, torch::Tensor z,
                        n_err.has_value() ? n_err->numel() : 0, x);
   check_gpu(op, x);
   c10::DeviceGuard guard(x.device());
+  torch::Tensor scratch;
+  void* wp = nullptr;
+  const long n = eval_distill_scratch(type, live, (int)C, (int)top);
+  if (n) {
+    scratch = torch::empty({n}, x.options().dtype(torch::kUInt8));
+    wp = scratch.data_ptr();
+  }
   eval_distill_launch(type, narrow ? ROW_BF16 : type, rows_in(x), ip, zp,
                       rows_out(err), sp, lp, np, (int)top, R, live, (int)C,
-                      (float)tau, cur_stream());
+                      (float)tau, wp, cur_stream());
 }
 
 }  // namespace

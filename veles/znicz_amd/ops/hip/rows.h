@@ -105,6 +105,9 @@ struct Pack {
   __device__ __forceinline__ void store(T* p) const {
     __builtin_memcpy(p, &raw, 16);
   }
+  __device__ __forceinline__ void store_once(T* p) const {
+    __builtin_nontemporal_store(raw, (u32x4_any*)p);
+  }
   // The compiler forgets what it knows of the elements, so that it takes
   // them apart again where they are used again, instead of holding them in
   // 32 bits each from one use to the other.

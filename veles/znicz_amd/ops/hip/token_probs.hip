@@ -93,20 +93,22 @@ struct Sums {
     um = M_MIN;
     s = w = 0.f;
   }
-  // the same sums to a larger m
+  // the same sums to a larger m (W: that of the entropy too)
+  template <bool W>
   __device__ __forceinline__ void raise(float to, float c) {
     const float um2 = fmaxf(to * c, M_MIN);
     const float by = um - um2, f = pow2(by);
-    w = f * fmaf(by, s, w);
+    if (W) w = f * fmaf(by, s, w);
     s *= f;
     m = to;
     um = um2;
   }
+  template <bool W>
   __device__ __forceinline__ void add(float x, float c) {
     const float u = fmaf(x, c, -um);
     const float e = pow2(u);
     s += e;
-    w = fmaf(e, fmaxf(u, U_MIN), w);
+    if (W) w = fmaf(e, fmaxf(u, U_MIN), w);
   }
 };
 
@@ -143,30 +145,23 @@ __device__ __forceinline__ bool is_far(float m, float c) {
 }
 
 // the waves' sums joined, in every thread; `tmp`: one for each wave
-template <int THREADS>
+template <bool W, int THREADS>
 __device__ __forceinline__ Sums join_block(Sums a, float c, Sums* tmp) {
   constexpr int WAVES = THREADS / WAVE;
-  a.raise(wave_max(a.m), c);
+  a.raise<W>(wave_max(a.m), c);
   a.s = wave_sum(a.s);
-  a.w = wave_sum(a.w);
+  if (W) a.w = wave_sum(a.w);
   if (WAVES == 1) return a;
   if ((threadIdx.x & (WAVE - 1)) == 0) tmp[threadIdx.x / WAVE] = a;
   __syncthreads();
-  float m = tmp[0].m;
-#pragma unroll
-  for (int i = 1; i < WAVES; ++i) m = fmaxf(m, tmp[i].m);
-  Sums t;
-  t.clear();
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) {
-    Sums b = tmp[i];
-    b.raise(m, c);
-    t.m = b.m;
-    t.um = b.um;
-    t.s += b.s;
-    t.w += b.w;
-  }
-  return t;
+  // (every wave joins them for itself, a lane to each)
+  const int lane = threadIdx.x & (WAVE - 1);
+  a.clear();
+  if (lane < WAVES) a = tmp[lane];
+  a.raise<W>(wave_max(a.m), c);
+  a.s = wave_sum(a.s);
+  if (W) a.w = wave_sum(a.w);
+  return a;
 }
 
 // Sums of a part of a row, to the exact C m: parts are joined by
@@ -200,9 +195,14 @@ __device__ __forceinline__ Row join_parts(const Part* p, int n, float c,
   t.s = wave_sum(f * a.s);
   t.w = wave_sum(f * fmaf(by, a.s, a.w));
   *first = wave_min(a.m == m ? a.first : 0x7fffffff);
+  // from the exact C m to M
+  if (m != -INFINITY && !is_far(m, c)) {
+    const float d = fmaf(m, c, -t.um), f = pow2(d);
+    t.w = f * fmaf(d, t.s, t.w);
+    t.s *= f;
+  }
   Row r;
   r.finish(t, c);
-  r.ln = log2_of(t.s) * LN2;             // (the parts are to the exact C m)
   return r;
 }
 
@@ -256,7 +256,7 @@ struct Held {
 // and no element is read twice.
 #define CHUNK 2
 
-template <typename T, int COUNT>
+template <bool W, typename T, int COUNT>
 __device__ __forceinline__ void add_packs(const Pack<T>* v, Sums& a, float c,
                                           float* high) {
   constexpr int N = Pack<T>::N;
@@ -272,17 +272,17 @@ __device__ __forceinline__ void add_packs(const Pack<T>* v, Sums& a, float c,
     if (high) high[i] = h;
     m = i ? max3(m, h, m) : h;
   }
-  a.raise(fmaxf(a.m, m), c);
+  a.raise<W>(fmaxf(a.m, m), c);
 #pragma unroll
   for (int i = 0; i < COUNT; ++i) {
     float e[N];
     v[i].get(e);
 #pragma unroll
-    for (int j = 0; j < N; ++j) a.add(e[j], c);
+    for (int j = 0; j < N; ++j) a.add<W>(e[j], c);
   }
 }
 
-template <typename T, int THREADS, int NV>
+template <bool W, typename T, int THREADS, int NV>
 __device__ __forceinline__ Sums held_sums(const Held<T, THREADS, NV>& h,
                                           int packs, float c, float* high) {
   constexpr int STEP = NV < CHUNK ? NV : CHUNK;
@@ -291,10 +291,10 @@ __device__ __forceinline__ Sums held_sums(const Held<T, THREADS, NV>& h,
 #pragma unroll
   for (int i = 0; i < NV; i += STEP) {
     if (i * THREADS >= packs) break;
-    add_packs<T, STEP>(h.v + i, a, c, high ? high + i : nullptr);
+    add_packs<W, T, STEP>(h.v + i, a, c, high ? high + i : nullptr);
   }
-  a.raise(fmaxf(a.m, h.rest), c);
-  a.add(h.rest, c);
+  a.raise<W>(fmaxf(a.m, h.rest), c);
+  a.add<W>(h.rest, c);
   return a;
 }
 
@@ -562,9 +562,9 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_held_k(
   Held<T, LP_THREADS, NV> h;
   h.load(x, cut);
   float high[NV];
-  Sums a = held_sums(h, cut.packs, LOG2E, high);
+  Sums a = held_sums<true>(h, cut.packs, LOG2E, high);
   sp.high[tid] = order_of(a.m);
-  a = join_block<LP_THREADS>(a, LOG2E, tmp);
+  a = join_block<true, LP_THREADS>(a, LOG2E, tmp);
   if (is_far(a.m, LOG2E)) a = far_sums(x, at.n, a.m, LOG2E, (float*)tmp);
   Row r;
   r.finish(a, LOG2E);
@@ -644,8 +644,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
   const T* body = x + cut.head;
   Sums a;
   a.clear();
-  a.raise(rest, LOG2E);
-  a.add(rest, LOG2E);
+  a.raise<true>(rest, LOG2E);
+  a.add<true>(rest, LOG2E);
   for (int b = 0; b < packs; b += STEP) {
     Pack<T> v[U];
     if (b + STEP <= packs) {
@@ -661,7 +661,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
       }
     }
     float high[U];
-    add_packs<T, U>(v, a, LOG2E, high);
+    add_packs<true, T, U>(v, a, LOG2E, high);
     if (TOP) {
       max_of_eight_lanes(high);
       // lane i of each eight has that of pack row i
@@ -672,7 +672,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
       if (i < U && g * GROUP < packs) groups[g] = h;
     }
   }
-  a = join_block<LP_THREADS>(a, LOG2E, tmp);
+  a = join_block<true, LP_THREADS>(a, LOG2E, tmp);
   if (is_far(a.m, LOG2E)) a = far_sums(x, at.n, a.m, LOG2E, (float*)tmp);
   Row r;
   r.finish(a, LOG2E);
@@ -777,122 +777,356 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_k(
 // ---------------------------------------------------------------------------
 // eval_distill
 // ---------------------------------------------------------------------------
+// q = softmax(z / tau) over the teacher's classes, p = softmax(x / tau) over
+// all;  loss = tau^2 sum q (ln q - ln p),  dloss/dx_j = tau (p_j - q_j).
+// The row is read once: it stays in registers until its sum is known.  The
+// teacher's classes are taken off the gradients in registers too, by the
+// threads that hold them, so that each gradient is written once.
 
-#define TP_THREADS 256
+struct DistillArgs {
+  RowsIn x;
+  const int* idx;
+  const float* z;
+  RowsOut err;
+  float* loss;
+  const int* labels;
+  int* n_err;
+  int top;
+  long rows, live;
+  int cols, size;
+  float tau, c;      // c = log2 e / tau
+  Part* parts;       // of split rows
+  float* xk;         // their logits of the teacher's classes
+};
 
-__device__ __forceinline__ Row plain_row(const Sums& a, float c) {
-  Row r;
-  r.finish(a, c);
-  return r;
+template <int THREADS>
+struct DistillSpace {
+  Sums tmp[THREADS / WAVE];
+  int id[MAX_TOP];           // -1: no class, or one that came before
+  float take[MAX_TOP];       // what it takes off its gradient
+  int next[MAX_TOP];         // the next one of the same thread
+  int head[THREADS];         // a thread's first one, or -1
+  unsigned where[THREADS];   // its packs with one; bit 31: its single element
+  int wrong, empty, first;
+};
+#define WHERE_MORE 30        // packs beyond those that are held
+#define WHERE_SINGLE 31
+
+// The teacher's side of a row; lane i of the first wave has its classes i
+// and i + 64.
+struct Teacher {
+  int id[2];
+  float z[2], x[2], q[2];
+  float zm, gs;
+  bool wrong;
+
+  __device__ __forceinline__ void load(const DistillArgs& a, long row) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = threadIdx.x + h * WAVE;
+      id[h] = -1;
+      z[h] = -INFINITY;
+      if (k < a.top) {
+        id[h] = a.idx[row * a.top + k];
+        z[h] = a.z[row * a.top + k];
+      }
+    }
+  }
+  // its logits in the student's row
+  template <typename T>
+  __device__ __forceinline__ void gather(const DistillArgs& a, const T* row) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      x[h] = id[h] >= 0 && id[h] < a.cols ? (float)row[id[h]] : 0.f;
+  }
+  __device__ __forceinline__ void gathered(const DistillArgs& a, long row) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = threadIdx.x + h * WAVE;
+      x[h] = k < a.top ? a.xk[row * a.top + k] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void softmax(const DistillArgs& a) {
+    bool w = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      w |= id[h] >= a.cols || (id[h] >= 0 && !(z[h] < INFINITY));
+      if (id[h] >= a.cols || z[h] == -INFINITY) id[h] = -1;
+      if (id[h] < 0) z[h] = -INFINITY;
+    }
+    wrong = __any(w);
+    zm = wave_max(fmaxf(z[0], z[1]));
+    float g[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      g[h] = id[h] >= 0 ? pow2((z[h] - zm) * a.c) : 0.f;
+    gs = wave_sum(g[0] + g[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) q[h] = g[h] / gs;
+  }
+  // tau sum q (ln q - ln p), of one lane
+  __device__ __forceinline__ float loss(const DistillArgs& a, const Row& r) {
+    const float apart = a.tau * (r.ln - log2_of(gs) * LN2);
+    float s = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (id[h] >= 0 && q[h] > 0.f)
+        s += q[h] * ((z[h] - zm) - (x[h] - r.m) + apart);
+    return s;
+  }
+};
+
+// the first class with the value m among those that this thread holds
+template <typename T, int THREADS, int NV>
+__device__ __forceinline__ int first_held(Held<T, THREADS, NV>& h, const T* x,
+                                          const Cut<T>& cut, float m) {
+  constexpr int N = Pack<T>::N;
+  const int tid = threadIdx.x;
+  int at = 0x7fffffff;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * THREADS >= cut.packs) break;
+    float e[N];
+    h.v[i].forget();
+    h.v[i].get(e);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (e[j] == m) at = min(at, cut.head + (i * THREADS + tid) * N + j);
+  }
+  for (int p = NV * THREADS + tid; p < cut.packs; p += THREADS)
+    for (int j = 0; j < N; ++j) {
+      const int k = cut.head + p * N + j;
+      if ((float)x[k] == m) at = min(at, k);
+    }
+  if (h.rest == m && cut.single >= 0) at = min(at, cut.single);
+  return at;
 }
 
-// Distillation: q = softmax(z / tau) over the teacher's classes, p =
-// softmax(x / tau) over all;
-//   loss = tau^2 sum q (ln q - ln p),  dloss/dx_j = tau (p_j - q_j).
-// One workgroup to a row.  A class that is named twice has the sum of both.
-template <typename T, typename O>
-__global__ __launch_bounds__(TP_THREADS) void distill_k(
-    RowsIn x_, const int* __restrict__ idx, const float* __restrict__ z,
-    RowsOut err_, float* __restrict__ loss, const int* __restrict__ labels,
-    int* __restrict__ n_err, int top, long rows, long live, int cols,
-    float tau) {
-  __shared__ float tmp[TP_THREADS / WAVE];
-  __shared__ int sid[MAX_TOP];
-  __shared__ float sq[MAX_TOP];
-  const int tid = threadIdx.x;
-  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
-    O* err = (O*)err_.p + row * err_.stride;
-    if (row >= live) {
-      for (int j = tid; j < cols; j += TP_THREADS) err[j] = from_f<O>(0.f);
-      if (tid == 0 && loss) loss[row] = 0.f;
-      continue;
-    }
-    const T* x = (const T*)x_.p + row * x_.stride;
-    const float c = LOG2E / tau;
-    float m = -INFINITY;
-    for (int j = tid; j < cols; j += TP_THREADS) m = fmaxf(m, (float)x[j]);
-    m = block_max(m, tmp);
-    Sums sums;
-    sums.clear();
-    sums.m = m;
-    sums.um = fmaxf(m * c, M_MIN);
-    const bool far = is_far(m, c);
-    for (int j = tid; j < cols; j += TP_THREADS) {
-      const float v = (float)x[j];
-      sums.s += pow2(far ? (v - m) * c : fmaf(v, c, -sums.um));
-    }
-    sums.s = block_sum(sums.s, tmp);
-    const Row r = plain_row(sums, c);
-    // the teacher's distribution: thread k has its k-th class
-    int id = -1;
-    float t = -INFINITY, xk = 0.f;
-    bool wrong = false;
-    if (tid < top) {
-      id = idx[row * top + tid];
-      if (id >= cols) {
-        wrong = true;
-      } else if (id >= 0) {
-        t = z[row * top + tid];
-        wrong = !(t < INFINITY);
-        xk = (float)x[id];
-      }
-      if (wrong || t == -INFINITY) id = -1;
-    }
-    const bool bad = __syncthreads_or(wrong) || r.bad;
-    const float zm = block_max(id >= 0 ? t : -INFINITY, tmp);
-    const float g = id >= 0 ? expf((t - zm) / tau) : 0.f;
-    const float gs = block_sum(g, tmp);
-    const bool lost = r.none || zm == -INFINITY;
-    float q = 0.f, part = 0.f;
-    if (!lost && id >= 0) {
-      q = g / gs;
-      // tau (ln q - ln p)
-      const float apart = (t - zm) - (xk - r.m) + tau * (r.ln - logf(gs));
-      part = q > 0.f ? q * apart : 0.f;
-    }
-    if (tid < top) {
-      sid[tid] = id;
-      sq[tid] = q;
-    }
-    part = block_sum(part, tmp);          // (and sid, sq are there)
-    if (tid == 0 && loss)
-      loss[row] = bad ? NAN : lost ? 0.f : tau * part;
-    if (labels) {
-      const int l = labels[row];
-      int first = 0x7fffffff;
-      for (int j = tid; j < cols; j += TP_THREADS)
-        if ((float)x[j] == r.m) {
-          first = j;
-          break;
-        }
+// sums of the packs beyond those that are held
+template <typename T, int THREADS, int NV>
+__device__ __forceinline__ void add_more(const T* x, const Cut<T>& cut,
+                                         Sums& a, float c) {
+  constexpr int N = Pack<T>::N;
+  for (int b = NV * THREADS; b < cut.packs; b += CHUNK * THREADS) {
+    Pack<T> v[CHUNK];
 #pragma unroll
-      for (int off = 32; off; off >>= 1)
-        first = min(first, __shfl_xor(first, off));
-      if ((tid & (WAVE - 1)) == 0) ((int*)tmp)[tid / WAVE] = first;
-      __syncthreads();
-      if (tid == 0 && l >= 0) {
-        for (int i = 1; i < TP_THREADS / WAVE; ++i)
-          first = min(first, ((int*)tmp)[i]);
-        if (bad || r.none || first != l) atomicAdd(n_err, 1);
+    for (int i = 0; i < CHUNK; ++i) {
+      const int p = b + i * THREADS + threadIdx.x;
+      v[i].fill(-INFINITY);
+      if (p < cut.packs) v[i].load(x + cut.head + (long)p * N);
+    }
+    add_packs<false, T, CHUNK>(v, a, c, nullptr);
+  }
+}
+
+template <typename T, typename O, int N>
+__device__ __forceinline__ void put_gradients(O* to, const float* g) {
+  if constexpr (__is_same(T, O)) {
+    Pack<O> v;
+    v.set(g);
+    v.store_once(to);
+  } else {
+    O t[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) t[j] = from_f<O>(g[j]);
+    __builtin_memcpy(to, t, sizeof(t));
+  }
+}
+
+// One workgroup to a row, or (JOINED) to a part of a row whose sums
+// distill_part_k has left.
+template <typename T, typename O, int THREADS, int NV, bool JOINED>
+__global__ __launch_bounds__(THREADS) void distill_k(DistillArgs a) {
+  __shared__ DistillSpace<THREADS> sp;
+  constexpr int N = Pack<T>::N;
+  const int tid = threadIdx.x;
+  const Place at(a.cols, a.size);
+  if (at.row >= a.rows) return;
+  O* err = (O*)a.err.p + at.row * a.err.stride + at.base;
+  if (at.row >= a.live) {
+    for (int j = tid; j < at.n; j += THREADS) err[j] = from_f<O>(0.f);
+    if (tid == 0 && at.base == 0 && a.loss) a.loss[at.row] = 0.f;
+    return;
+  }
+  const bool leads = tid < WAVE;
+  Teacher t;
+  if (leads) t.load(a, at.row);
+  const T* row = (const T*)a.x.p + at.row * a.x.stride;
+  const T* x = row + at.base;
+  const Cut<T> cut(x, at.n);
+  Held<T, THREADS, NV> h;
+  h.load(x, cut);
+  if (leads) {
+    if (JOINED)
+      t.gathered(a, at.row);
+    else
+      t.gather(a, row);
+    t.softmax(a);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sp.id[tid + i * WAVE] = t.id[i];
+      sp.take[tid + i * WAVE] = t.q[i];
+    }
+    if (tid == 0) {
+      sp.wrong = t.wrong;
+      sp.empty = t.zm == -INFINITY;
+      sp.first = 0x7fffffff;
+    }
+  }
+  sp.head[tid] = -1;
+  sp.where[tid] = 0;
+  Row r;
+  int first = 0x7fffffff;
+  if (JOINED) {
+    r = join_parts(a.parts + at.row * gridDim.x, gridDim.x, a.c, &first);
+    __syncthreads();
+  } else {
+    Sums s = held_sums<false>(h, cut.packs, a.c, nullptr);
+    add_more<T, THREADS, NV>(x, cut, s, a.c);
+    const float own = s.m;
+    s = join_block<false, THREADS>(s, a.c, sp.tmp);
+    if (is_far(s.m, a.c)) s = far_sums(x, at.n, s.m, a.c, (float*)sp.tmp);
+    r.finish(s, a.c);
+    if (a.labels && own == r.m && !r.none)
+      atomicMin(&sp.first, first_held(h, x, cut, r.m));
+  }
+  const bool bad = r.bad || sp.wrong;
+  const bool lost = r.none || sp.empty;
+  if (leads && !bad && !lost) {
+    const float loss = wave_sum(t.loss(a, r));
+    if (tid == 0 && at.base == 0 && a.loss) a.loss[at.row] = a.tau * loss;
+    // what each class takes off, all its places together
+    float sum[2];
+    bool again[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sum[i] = 0.f;
+      again[i] = t.id[i] < 0;
+      for (int j = 0; j < a.top; ++j) {
+        const bool same = sp.id[j] == t.id[i];
+        sum[i] += same ? sp.take[j] : 0.f;
+        again[i] |= same && j < tid + i * WAVE;
       }
     }
-    // err may lie over x: what is read of x is read before
-    float mine = 0.f, sum = 0.f;
-    if (id >= 0) {
-      mine = pow2(r.u(xk));
-      for (int k = 0; k < top; ++k)
-        if (sid[k] == id) sum += sq[k];
+    // (one wave: all its reads are before its writes)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int k = tid + i * WAVE;
+      const int j = t.id[i] - at.base;
+      if (again[i] || j < 0 || j >= at.n) {
+        sp.id[k] = -1;
+      } else {
+        sp.id[k] = j;
+        sp.take[k] = a.tau * sum[i];
+        const int p = j - cut.head, tail = cut.packs * N;
+        int owner, bit = WHERE_SINGLE;
+        if (p < 0) {
+          owner = j;
+        } else if (p >= tail) {
+          owner = N + p - tail;
+        } else {
+          owner = p / N % THREADS;
+          bit = min(p / N / THREADS, NV < WHERE_MORE ? NV : WHERE_MORE);
+          if (bit == NV) bit = WHERE_MORE;
+        }
+        sp.next[k] = atomicExch(&sp.head[owner], k);
+        atomicOr(&sp.where[owner], 1u << bit);
+      }
     }
-    __syncthreads();
-    const float a = bad ? NAN : lost ? 0.f : tau / r.s;
-    for (int j = tid; j < cols; j += TP_THREADS) {
-      const float e = pow2(r.u((float)x[j]));
-      err[j] = from_f<O>(lost && !bad ? 0.f : a * e);
+  } else if (tid == 0 && at.base == 0 && a.loss) {
+    a.loss[at.row] = bad ? NAN : 0.f;
+  }
+  __syncthreads();
+  if (a.labels && tid == 0 && at.base == 0) {
+    const int l = a.labels[at.row];
+    if (!JOINED) first = sp.first;
+    if (l >= 0 && (bad || r.none || first != l)) atomicAdd(a.n_err, 1);
+  }
+
+  const float scale = bad ? NAN : lost ? 0.f : a.tau / r.s;
+  if (r.far) {
+    // (all classes one by one; the places of the teacher's are searched)
+    for (int j = tid; j < at.n; j += THREADS) {
+      float g = bad ? NAN : lost ? 0.f : scale * pow2(r.u((float)x[j]));
+      if (!bad && !lost)
+        for (int k = 0; k < a.top; ++k)
+          if (sp.id[k] == j) g -= sp.take[k];
+      err[j] = from_f<O>(g);
     }
+    return;
+  }
+  const unsigned where = sp.where[tid];
+  // gradients of a pack; `some`: with classes of the teacher's
+  auto pack = [&](const Pack<T>& v, int p, bool some) {
+    float g[N];
+    v.get(g);
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] = scale * pow2(fmaf(g[j], a.c, -r.um));
+    const int j = cut.head + p * N;
+    if (some) {
+      for (int k = sp.head[tid]; k >= 0; k = sp.next[k]) {
+        const int d = sp.id[k] - j;
+        const float by = sp.take[k];
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] -= d == i ? by : 0.f;
+      }
+    }
+    put_gradients<T, O, N>(err + j, g);
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * THREADS >= cut.packs) break;
+    const int p = i * THREADS + tid;
+    h.v[i].forget();
+    if (p < cut.packs) pack(h.v[i], p, where >> i & 1);
+  }
+  for (int p = NV * THREADS + tid; p < cut.packs; p += THREADS) {
+    Pack<T> v;
+    v.load(x + cut.head + (long)p * N);
+    pack(v, p, where >> WHERE_MORE & 1);
+  }
+  if (cut.single >= 0) {
+    float g = scale * pow2(fmaf(h.rest, a.c, -r.um));
+    if (where >> WHERE_SINGLE & 1)
+      for (int k = sp.head[tid]; k >= 0; k = sp.next[k])
+        g -= sp.id[k] == cut.single ? sp.take[k] : 0.f;
+    err[cut.single] = from_f<O>(g);
+  }
+}
+
+// sums of a part of a row, and the row's logits of the teacher's classes
+template <typename T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS) void distill_part_k(DistillArgs a) {
+  __shared__ Sums tmp[THREADS / WAVE];
+  __shared__ int first;
+  const Place at(a.cols, a.size);
+  if (at.row >= a.live) return;
+  const T* row = (const T*)a.x.p + at.row * a.x.stride;
+  const T* x = row + at.base;
+  if (at.base == 0)
+    for (int k = threadIdx.x; k < a.top; k += THREADS) {
+      const int id = a.idx[at.row * a.top + k];
+      a.xk[at.row * a.top + k] =
+          id >= 0 && id < a.cols ? (float)row[id] : 0.f;
+    }
+  if (threadIdx.x == 0) first = 0x7fffffff;
+  const Cut<T> cut(x, at.n);
+  Held<T, THREADS, NV> h;
+  h.load(x, cut);
+  Sums s = held_sums<false>(h, cut.packs, a.c, nullptr);
+  add_more<T, THREADS, NV>(x, cut, s, a.c);
+  const float own = s.m;
+  s = join_block<false, THREADS>(s, a.c, tmp);
+  if (is_far(s.m, a.c)) s = far_sums(x, at.n, s.m, a.c, (float*)tmp);
+  if (a.labels) {
+    if (own == s.m) atomicMin(&first, first_held(h, x, cut, s.m));
     __syncthreads();
-    if (id >= 0 && !bad && !lost)
-      err[id] = from_f<O>(fmaf(a, mine, -tau * sum));
-    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const int at_first = a.labels && first < at.n ? at.base + first
+                                                  : 0x7fffffff;
+    a.parts[at.item] = part_of(s, a.c, at_first);
   }
 }
 
@@ -1006,22 +1240,79 @@ void token_logprobs_launch(int type, RowsIn x, const int* labels,
 #undef RUN
 }
 
+// How a call is laid out: parts of a row, elements of a part, threads and
+// packs of a thread
+struct DistillPlan {
+  int split, size, threads, nv;
+};
+
+static DistillPlan distill_plan(int type, long rows, int cols) {
+  const int n = type == ROW_F32 ? 4 : 8;
+  DistillPlan p{1, cols, 256, 1};
+  const long least = 256 * 4 * n;
+  long split = 1;
+  if (rows < 256)
+    while (split < 64 && rows * split < 512 && cols / (split + 1) >= least)
+      ++split;
+  if (split > 1) {
+    long size = (cols + split - 1) / split;
+    p.size = (int)((size + n - 1) / n * n);
+    p.split = (cols + p.size - 1) / p.size;
+  }
+  if ((long)p.size > 256 * 8 * n) p.threads = 1024;
+  while (p.nv < (p.threads == 256 ? 8 : 16) &&
+         (long)p.threads * p.nv * n < p.size)
+    p.nv *= 2;
+  return p;
+}
+
+// bytes that eval_distill_launch needs at `scratch`
+long eval_distill_scratch(int type, long live, int cols, int top) {
+  const DistillPlan p = distill_plan(type, live, cols);
+  if (p.split == 1) return 0;
+  return live * (p.split * (long)sizeof(Part) + top * (long)sizeof(float));
+}
+
+template <typename T, typename O>
+static void distill_run(DistillArgs a, DistillPlan p, hipStream_t s) {
+#define CASE(THREADS, NV)                                                    \
+  if (p.threads == THREADS && p.nv == NV) {                                  \
+    if (p.split == 1) {                                                      \
+      hipLaunchKernelGGL(                                                    \
+          HIP_KERNEL_NAME(distill_k<T, O, THREADS, NV, false>),              \
+          parts_grid(1, a.rows), dim3(THREADS), 0, s, a);                    \
+    } else {                                                                 \
+      if (a.live)                                                            \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_part_k<T, THREADS, NV>),  \
+                           parts_grid(p.split, a.live), dim3(THREADS), 0, s, \
+                           a);                                               \
+      hipLaunchKernelGGL(                                                    \
+          HIP_KERNEL_NAME(distill_k<T, O, THREADS, NV, true>),               \
+          parts_grid(p.split, a.rows), dim3(THREADS), 0, s, a);              \
+    }                                                                        \
+  }
+  CASE(256, 1) CASE(256, 2) CASE(256, 4) CASE(256, 8)
+  CASE(1024, 4) CASE(1024, 8) CASE(1024, 16)
+#undef CASE
+  HIP_CHECK_LAST();
+}
+
 void eval_distill_launch(int type, int err_type, RowsIn x, const int* idx,
                          const float* z, RowsOut err, float* loss,
                          const int* labels, int* n_err, int top, long rows,
-                         long live, int cols, float tau, hipStream_t s) {
+                         long live, int cols, float tau, void* scratch,
+                         hipStream_t s) {
   if (rows == 0) return;
-#define RUN2(T, O)                                                           \
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_k<T, O>), dim3(row_grid(rows)), \
-                     dim3(TP_THREADS), 0, s, x, idx, z, err, loss, labels,   \
-                     n_err, top, rows, live, cols, tau)
-#define RUN(T) RUN2(T, T)
+  const DistillPlan p = distill_plan(type, live, cols);
+  Part* parts = (Part*)scratch;
+  DistillArgs a{x, idx, z, err, loss, labels, n_err, top, rows, live, cols,
+                p.size, tau, LOG2E / tau, parts,
+                p.split > 1 ? (float*)(parts + live * p.split) : nullptr};
+#define RUN(T) distill_run<T, T>(a, p, s)
   if (type == ROW_F32 && err_type == ROW_BF16) {
-    RUN2(float, bf16_t);
+    distill_run<float, bf16_t>(a, p, s);
   } else {
     ROW_TYPE_SWITCH(type, RUN)
   }
 #undef RUN
-#undef RUN2
-  HIP_CHECK_LAST();
 }
