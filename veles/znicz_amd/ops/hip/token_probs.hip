@@ -241,13 +241,15 @@ struct Held {
 
   __device__ __forceinline__ void load(const T* x, const Cut<T>& cut) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      v[i].fill(-INFINITY);
-      // (one offset for all, from bases that are the same for a wave)
-      if (i * THREADS + (int)threadIdx.x < cut.packs)
-        v[i].load_once(x + cut.head + i * THREADS * N + threadIdx.x * N);
-    }
+    for (int i = 0; i < NV; ++i) load_pack(i, x, cut);
     rest = cut.load_single(x);
+  }
+  __device__ __forceinline__ void load_pack(int i, const T* x,
+                                            const Cut<T>& cut) {
+    v[i].fill(-INFINITY);
+    // (one offset for all, from bases that are the same for a wave)
+    if (i * THREADS + (int)threadIdx.x < cut.packs)
+      v[i].load_once(x + cut.head + i * THREADS * N + threadIdx.x * N);
   }
 };
 
@@ -442,7 +444,7 @@ __device__ __forceinline__ float share_bound(TopSpace<THREADS>& sp, int top) {
 // itself, then among the classes that hold it the last that is needed, by
 // halving; the part x[0..n) is read from the caches each time.
 template <typename T, int THREADS>
-__device__ __noinline__ void thin_out(const T* x, int n, int base, int top,
+__device__ __forceinline__ void thin_out(const T* x, int n, int base, int top,
                                       TopSpace<THREADS>& sp) {
   const int tid = threadIdx.x;
   int lo = sp.bound, hi = 0x7f800000;
@@ -510,7 +512,7 @@ __device__ __forceinline__ void put_top(const PartOut& p, long row, long item,
 
 // Where u = C x - M does not do: the sums of the part x[0..n) once more
 template <typename T>
-__device__ __noinline__ Sums far_sums(const T* x, int n, float m, float c,
+__device__ __forceinline__ Sums far_sums(const T* x, int n, float m, float c,
                                       float* tmp) {
   Sums a;
   a.m = m;
@@ -801,7 +803,6 @@ struct DistillArgs {
 
 template <int THREADS>
 struct DistillSpace {
-  Sums tmp[THREADS / WAVE];
   int id[MAX_TOP];           // -1: no class, or one that came before
   float take[MAX_TOP];       // what it takes off its gradient
   int next[MAX_TOP];         // the next one of the same thread
@@ -864,7 +865,59 @@ struct Teacher {
 #pragma unroll
     for (int h = 0; h < 2; ++h) q[h] = g[h] / gs;
   }
-  // tau sum q (ln q - ln p), of one lane
+  // Leaves what each class takes off its gradient, all places of a class
+  // together, with the thread that holds the element of x[0..n).
+  template <typename T, int THREADS, int NV>
+  __device__ __forceinline__ void place(const DistillArgs& a, int base, int n,
+                                        const Cut<T>& cut,
+                                        DistillSpace<THREADS>& sp) {
+    constexpr int N = Pack<T>::N;
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sp.id[tid + h * WAVE] = id[h];
+      sp.take[tid + h * WAVE] = q[h];
+    }
+    __builtin_amdgcn_wave_barrier();
+    float sum[2] = {0.f, 0.f};
+    bool again[2] = {id[0] < 0, id[1] < 0};
+#pragma unroll 4
+    for (int j = 0; j < (a.top + 3) / 4 * 4; ++j) {
+      const int other = sp.id[j];
+      const float share = sp.take[j];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool same = other == id[h];
+        sum[h] += same ? share : 0.f;
+        again[h] |= same && j < tid + h * WAVE;
+      }
+    }
+    // (one wave: all its reads are before its writes)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = tid + h * WAVE;
+      const int j = id[h] - base;
+      sp.id[k] = -1;
+      if (again[h] || j < 0 || j >= n) continue;
+      sp.id[k] = j;
+      sp.take[k] = a.tau * sum[h];
+      const int p = j - cut.head, tail = cut.packs * N;
+      int owner, bit = WHERE_SINGLE;
+      if (p < 0) {
+        owner = j;
+      } else if (p >= tail) {
+        owner = N + p - tail;
+      } else {
+        owner = p / N % THREADS;
+        bit = p / N / THREADS;
+        if (bit >= NV) bit = WHERE_MORE;
+      }
+      sp.next[k] = atomicExch(&sp.head[owner], k);
+      atomicOr(&sp.where[owner], 1u << bit);
+    }
+  }
+  // tau sum q (ln q - ln p)
   __device__ __forceinline__ float loss(const DistillArgs& a, const Row& r) {
     const float apart = a.tau * (r.ln - log2_of(gs) * LN2);
     float s = 0.f;
@@ -872,7 +925,7 @@ struct Teacher {
     for (int h = 0; h < 2; ++h)
       if (id[h] >= 0 && q[h] > 0.f)
         s += q[h] * ((z[h] - zm) - (x[h] - r.m) + apart);
-    return s;
+    return wave_sum(s);
   }
 };
 
@@ -934,10 +987,12 @@ __device__ __forceinline__ void put_gradients(O* to, const float* g) {
 }
 
 // One workgroup to a row, or (JOINED) to a part of a row whose sums
-// distill_part_k has left.
+// distill_part_k has left.  The teacher's side is done by the first wave
+// while the row is under way.
 template <typename T, typename O, int THREADS, int NV, bool JOINED>
 __global__ __launch_bounds__(THREADS) void distill_k(DistillArgs a) {
   __shared__ DistillSpace<THREADS> sp;
+  __shared__ Sums tmp[THREADS / WAVE];
   constexpr int N = Pack<T>::N;
   const int tid = threadIdx.x;
   const Place at(a.cols, a.size);
@@ -949,32 +1004,29 @@ __global__ __launch_bounds__(THREADS) void distill_k(DistillArgs a) {
     return;
   }
   const bool leads = tid < WAVE;
-  Teacher t;
-  if (leads) t.load(a, at.row);
   const T* row = (const T*)a.x.p + at.row * a.x.stride;
   const T* x = row + at.base;
   const Cut<T> cut(x, at.n);
+  Teacher t;
+  if (leads) t.load(a, at.row);
   Held<T, THREADS, NV> h;
   h.load(x, cut);
+  sp.head[tid] = -1;
+  sp.where[tid] = 0;
+  __syncthreads();
   if (leads) {
     if (JOINED)
       t.gathered(a, at.row);
     else
       t.gather(a, row);
     t.softmax(a);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sp.id[tid + i * WAVE] = t.id[i];
-      sp.take[tid + i * WAVE] = t.q[i];
-    }
+    t.place<T, THREADS, NV>(a, at.base, at.n, cut, sp);
     if (tid == 0) {
       sp.wrong = t.wrong;
       sp.empty = t.zm == -INFINITY;
       sp.first = 0x7fffffff;
     }
   }
-  sp.head[tid] = -1;
-  sp.where[tid] = 0;
   Row r;
   int first = 0x7fffffff;
   if (JOINED) {
@@ -984,64 +1036,27 @@ __global__ __launch_bounds__(THREADS) void distill_k(DistillArgs a) {
     Sums s = held_sums<false>(h, cut.packs, a.c, nullptr);
     add_more<T, THREADS, NV>(x, cut, s, a.c);
     const float own = s.m;
-    s = join_block<false, THREADS>(s, a.c, sp.tmp);
-    if (is_far(s.m, a.c)) s = far_sums(x, at.n, s.m, a.c, (float*)sp.tmp);
+    s = join_block<false, THREADS>(s, a.c, tmp);
+    if (is_far(s.m, a.c)) s = far_sums(x, at.n, s.m, a.c, (float*)tmp);
     r.finish(s, a.c);
-    if (a.labels && own == r.m && !r.none)
-      atomicMin(&sp.first, first_held(h, x, cut, r.m));
+    if (a.labels) {
+      if (own == r.m && !r.none)
+        atomicMin(&sp.first, first_held(h, x, cut, r.m));
+      __syncthreads();
+      first = sp.first;
+    }
   }
   const bool bad = r.bad || sp.wrong;
   const bool lost = r.none || sp.empty;
-  if (leads && !bad && !lost) {
-    const float loss = wave_sum(t.loss(a, r));
-    if (tid == 0 && at.base == 0 && a.loss) a.loss[at.row] = a.tau * loss;
-    // what each class takes off, all its places together
-    float sum[2];
-    bool again[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sum[i] = 0.f;
-      again[i] = t.id[i] < 0;
-      for (int j = 0; j < a.top; ++j) {
-        const bool same = sp.id[j] == t.id[i];
-        sum[i] += same ? sp.take[j] : 0.f;
-        again[i] |= same && j < tid + i * WAVE;
+  if (leads && at.base == 0) {
+    const float loss = bad ? NAN : lost ? 0.f : a.tau * t.loss(a, r);
+    if (tid == 0) {
+      if (a.loss) a.loss[at.row] = loss;
+      if (a.labels) {
+        const int l = a.labels[at.row];
+        if (l >= 0 && (bad || r.none || first != l)) atomicAdd(a.n_err, 1);
       }
     }
-    // (one wave: all its reads are before its writes)
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int k = tid + i * WAVE;
-      const int j = t.id[i] - at.base;
-      if (again[i] || j < 0 || j >= at.n) {
-        sp.id[k] = -1;
-      } else {
-        sp.id[k] = j;
-        sp.take[k] = a.tau * sum[i];
-        const int p = j - cut.head, tail = cut.packs * N;
-        int owner, bit = WHERE_SINGLE;
-        if (p < 0) {
-          owner = j;
-        } else if (p >= tail) {
-          owner = N + p - tail;
-        } else {
-          owner = p / N % THREADS;
-          bit = min(p / N / THREADS, NV < WHERE_MORE ? NV : WHERE_MORE);
-          if (bit == NV) bit = WHERE_MORE;
-        }
-        sp.next[k] = atomicExch(&sp.head[owner], k);
-        atomicOr(&sp.where[owner], 1u << bit);
-      }
-    }
-  } else if (tid == 0 && at.base == 0 && a.loss) {
-    a.loss[at.row] = bad ? NAN : 0.f;
-  }
-  __syncthreads();
-  if (a.labels && tid == 0 && at.base == 0) {
-    const int l = a.labels[at.row];
-    if (!JOINED) first = sp.first;
-    if (l >= 0 && (bad || r.none || first != l)) atomicAdd(a.n_err, 1);
   }
 
   const float scale = bad ? NAN : lost ? 0.f : a.tau / r.s;
@@ -1056,7 +1071,7 @@ __global__ __launch_bounds__(THREADS) void distill_k(DistillArgs a) {
     }
     return;
   }
-  const unsigned where = sp.where[tid];
+  const unsigned where = lost ? 0 : sp.where[tid];
   // gradients of a pack; `some`: with classes of the teacher's
   auto pack = [&](const Pack<T>& v, int p, bool some) {
     float g[N];
@@ -1259,10 +1274,10 @@ static DistillPlan distill_plan(int type, long rows, int cols) {
     p.size = (int)((size + n - 1) / n * n);
     p.split = (cols + p.size - 1) / p.size;
   }
-  if ((long)p.size > 256 * 8 * n) p.threads = 1024;
-  while (p.nv < (p.threads == 256 ? 8 : 16) &&
-         (long)p.threads * p.nv * n < p.size)
-    p.nv *= 2;
+  p.threads = (long)p.size <= 256 * 16 * n ? 256
+              : (long)p.size <= 512 * 16 * n ? 512 : 1024;
+  p.nv = p.threads > 256 ? 16 : 1;
+  while (p.nv < 16 && (long)p.threads * p.nv * n < p.size) p.nv *= 2;
   return p;
 }
 
@@ -1291,8 +1306,8 @@ static void distill_run(DistillArgs a, DistillPlan p, hipStream_t s) {
           parts_grid(p.split, a.rows), dim3(THREADS), 0, s, a);              \
     }                                                                        \
   }
-  CASE(256, 1) CASE(256, 2) CASE(256, 4) CASE(256, 8)
-  CASE(1024, 4) CASE(1024, 8) CASE(1024, 16)
+  CASE(256, 1) CASE(256, 2) CASE(256, 4) CASE(256, 8) CASE(256, 16)
+  CASE(512, 16) CASE(1024, 16)
 #undef CASE
   HIP_CHECK_LAST();
 }
