@@ -84,7 +84,7 @@ void lrn_bwd_launch(const unsigned short*, const unsigned short*,
 // from layer_norm.hip
 void layer_norm_fwd_launch(int, RowsIn, RowsOut, const float*, const float*,
                            float*, float*, long, int, float, hipStream_t);
-long layer_norm_bwd_scratch(int, long, int);
+long layer_norm_bwd_scratch(long, int);
 void layer_norm_bwd_launch(int, RowsIn, RowsIn, const float*, const float*,
                            const float*, RowsOut, float*, float*, bool,
                            float*, long, int, hipStream_t);
@@ -606,7 +606,7 @@ void layer_norm_bwd(torch::Tensor dy, torch::Tensor x, Opt w,
   c10::DeviceGuard guard(x.device());
   torch::Tensor part;
   float* pp = nullptr;
-  const long n = dwp || dbp ? layer_norm_bwd_scratch(type, R, (int)C) : 0;
+  const long n = dwp || dbp ? layer_norm_bwd_scratch(R, (int)C) : 0;
   if (n) {
     part = torch::empty({n}, x.options().dtype(torch::kFloat32));
     pp = part.data_ptr<float>();
