@@ -14,6 +14,13 @@
 #define LN_PARTS 256
 // workgroups of 256 threads that a backward pass of teams has at most
 #define LN_BLOCKS 768
+#ifndef LN_RA
+#define LN_RA 2
+#define LN_RB 2
+#define LN_RC 1
+#define LN_FB 2048
+#define LN_ONCE 0
+#endif
 
 // one workgroup to a row; the row is read three times, from the caches
 // after the first
@@ -151,37 +158,51 @@ struct TeamSum {
         } else {
           v[i] += other_lane<0xb1>(v[i]);
           v[i] += other_lane<0x4e>(v[i]);
-          if (TEAM > 4) {
-            v[i] += other_lane<0x141>(v[i]);
-            v[i] += other_lane<0x140>(v[i]);
-          }
+          if (TEAM > 4) v[i] += other_lane<0x141>(v[i]);
+          if (TEAM > 8) v[i] += other_lane<0x140>(v[i]);
+          if (TEAM > 16) v[i] += __shfl_xor(v[i], 16);
         }
       }
     } else {
+      // a wave's sum comes to its last lane; the waves' are joined by a lane
+      // to each
       constexpr int WAVES = TEAM / WAVE;
       float* t = tmp + turn * R * WAVES;
       turn ^= 1;
+      const int lane = threadIdx.x & (WAVE - 1);
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        const float w = wave_sum(v[i]);
-        if ((threadIdx.x & (WAVE - 1)) == 0) t[i * WAVES + threadIdx.x / WAVE] = w;
+        const float w = wave_sum_last(v[i]);
+        if (lane == WAVE - 1) t[i * WAVES + threadIdx.x / WAVE] = w;
       }
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        v[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < WAVES; ++k) v[i] += t[i * WAVES + k];
+        v[i] = t[i * WAVES + lane % WAVES];
+        v[i] += other_lane<0xb1>(v[i]);
+        if (WAVES > 2) v[i] += other_lane<0x4e>(v[i]);
+        if (WAVES > 4) v[i] += other_lane<0x141>(v[i]);
+        if (WAVES > 8) v[i] += other_lane<0x140>(v[i]);
       }
     }
   }
 };
 
+// 1 / sqrt(v): one unit in the last place (v_rsq_f32, which takes numbers
+// below 2^-126 for 0)
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const bool small = v < 0x1p-100f;
+  const float r = __builtin_amdgcn_rsqf(small ? v * 0x1p100f : v);
+  return small ? r * 0x1p50f : r;
+}
+
 // Where a lane's packs of a row lie.  The last pack of a row that is no
 // whole number of packs ends with the row, so that its first elements are
-// the pack's before, too: `lo` of them count there.  A row shorter than a
-// pack is read one by one.
-template <typename T, int TEAM, int NV>
+// the pack's before, too; a lane beyond the last pack has that one again.
+// Both are loaded and stored like any other (the same values to the same
+// place), which spares the branches, and are left out of the sums.  A row
+// shorter than a pack (TINY) is read and written one by one.
+template <typename T, int TEAM, int NV, bool TINY>
 struct Slots {
   static constexpr int N = Pack<T>::N;
   int lane, cols, packs;
@@ -196,35 +217,33 @@ struct Slots {
   }
   __device__ __forceinline__ int at(int i) const {
     const int j = (i * TEAM + lane) * N;
-    return max(min(j, cols - N), 0);
+    return TINY ? 0 : min(j, cols - N);
   }
   // whether element k of pack i is this pack's own
-  template <bool EXACT>
   __device__ __forceinline__ bool own(int i, int k) const {
-    if (EXACT) return has(i);
     const int j = (i * TEAM + lane) * N;
     return has(i) && at(i) + k >= j && at(i) + k < cols;
   }
   __device__ __forceinline__ void load(Pack<T>& v, const T* row, int i) const {
-    if (cols >= N) {
-      v.load(row + at(i));
-    } else {
+    if (TINY) {
       float e[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) e[k] = k < cols ? (float)row[k] : 0.f;
       v.set(e);
+    } else {
+      v.load(row + at(i));
     }
   }
   __device__ __forceinline__ void store(const Pack<T>& v, T* row,
                                         int i) const {
-    if (cols >= N) {
-      v.store(row + at(i));
-    } else {
+    if (TINY) {
       T e[N];
       __builtin_memcpy(e, &v.raw, 16);
 #pragma unroll
       for (int k = 0; k < N; ++k)
         if (k < cols) row[k] = e[k];
+    } else {
+      v.store(row + at(i));
     }
   }
   // parameters of the lane's columns
@@ -233,55 +252,81 @@ struct Slots {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int j = at(i) + k;
-        v[i * N + k] = p && has(i) && j < cols ? p[j] : none;
-      }
+      for (int k = 0; k < N; ++k)
+        v[i * N + k] = p && (!TINY || k < cols) ? p[at(i) + k] : none;
   }
 };
 
-template <typename T, int THREADS, int TEAM, int NV, int R, bool EXACT>
+// The rows of a team: from `start`, `step` apart R at a time.  All lanes of
+// a wave (a workgroup, where it is the team) make the same number of steps.
+template <int THREADS, int TEAM, int R>
+struct Steps {
+  long start, teams;
+  int mine;        // this lane's team among those of its wave
+
+  __device__ __forceinline__ Steps() {
+    constexpr int TEAMS = THREADS / TEAM;
+    teams = (long)gridDim.x * TEAMS;
+    start = (long)blockIdx.x * TEAMS;
+    if (TEAM < THREADS)
+      start += __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) *
+               (TEAM < WAVE ? WAVE / TEAM : 1);
+    mine = TEAM < WAVE ? (threadIdx.x & (WAVE - 1)) / TEAM : 0;
+  }
+  // whether all rows of the step from `first` exist
+  __device__ __forceinline__ bool full(long first, long rows) const {
+    return first + (R - 1) * teams + (TEAM < WAVE ? WAVE / TEAM - 1 : 0) <
+           rows;
+  }
+};
+
+// All loads so far have arrived.  (Before a loop whose first loads were
+// issued outside, so that within it the compiler counts those of the loop
+// alone.)
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt 0
+}
+
+// In each step the next one's loads come before this one's stores: memory
+// operations are waited for in their order, and what waits for a load would
+// otherwise wait for stores to reach memory.  For the same reason nothing
+// after those loads is on a condition; the last step is apart.
+template <typename T, int THREADS, int TEAM, int NV, int R, bool EXACT,
+          bool TINY>
 __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
     RowsIn x_, RowsOut y_, const float* __restrict__ w,
     const float* __restrict__ b, float* __restrict__ mean,
     float* __restrict__ rstd, long rows, int cols, float eps) {
-  constexpr int N = Pack<T>::N, TEAMS = THREADS / TEAM;
+  constexpr int N = Pack<T>::N;
   __shared__ float tmp[2 * R * (THREADS / WAVE)];
   TeamSum<TEAM, R> sum{tmp, 0};
-  const Slots<T, TEAM, NV> at(cols);
+  const Slots<T, TEAM, NV, TINY> at(cols);
+  const Steps<THREADS, TEAM, R> steps;
   float gain[NV * N], shift[NV * N];
-  at.load_param(gain, w, 1.f);
-  at.load_param(shift, b, 0.f);
-  const long teams = (long)gridDim.x * TEAMS;
   const float per = 1.f / cols;
-  // (all lanes of a wave make the same number of steps)
-  for (long first = (long)blockIdx.x * TEAMS + (TEAM < THREADS
-                        ? (int)threadIdx.x / WAVE * (WAVE / TEAM) : 0);
-       first < rows; first += teams * R) {
-    const long row0 =
-        first + (TEAM < WAVE ? (threadIdx.x & (WAVE - 1)) / TEAM : 0);
-    Pack<T> v[R][NV];
+  Pack<T> v[R][NV];
+  auto load = [&](long row0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long row = row0 + r * teams;
-      const T* x = (const T*)x_.p + row * x_.stride;
+      const long row = min(row0 + r * steps.teams, rows - 1);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        v[r][i].fill(0.f);
-        if (row < rows && at.has(i)) at.load(v[r][i], x, i);
-      }
+      for (int i = 0; i < NV; ++i)
+        at.load(v[r][i], (const T*)x_.p + row * x_.stride, i);
     }
+  };
+  auto step = [&](long row0, bool last) {
     float mu[R], rs[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       mu[r] = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        float e[N];
+        float e[N], q = 0.f;
         v[r][i].get(e);
 #pragma unroll
         for (int k = 0; k < N; ++k)
-          mu[r] += EXACT || at.template own<EXACT>(i, k) ? e[k] : 0.f;
+          q += EXACT || at.own(i, k) ? e[k] : 0.f;
+        mu[r] += at.has(i) ? q : 0.f;
       }
     }
     sum(mu);
@@ -297,7 +342,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           float d = e[k] - mu[r];
-          if (!EXACT) d = at.template own<EXACT>(i, k) ? d : 0.f;
+          if (!EXACT) d = at.own(i, k) ? d : 0.f;
           q = fmaf(d, d, q);
         }
         rs[r] += at.has(i) ? q : 0.f;
@@ -306,10 +351,13 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
     sum(rs);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long row = row0 + r * teams;
-      rs[r] = 1.f / sqrtf(fmaf(rs[r], per, eps));
-      if (row >= rows) continue;
-      T* y = (T*)y_.p + row * y_.stride;
+      const long row = row0 + r * steps.teams;
+      rs[r] = inv_sqrt(fmaf(rs[r], per, eps));
+      if (at.lane == 0 && mean && row < rows) mean[row] = mu[r];
+      if (at.lane == 0 && rstd && row < rows) rstd[row] = rs[r];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         float e[N];
@@ -320,68 +368,78 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
           e[k] = fmaf((e[k] - mu[r]) * rs[r], gain[i * N + k],
                       shift[i * N + k]);
         v[r][i].set(e);
-        if (at.has(i)) at.store(v[r][i], y, i);
       }
-      if (at.lane == 0) {
-        if (mean) mean[row] = mu[r];
-        if (rstd) rstd[row] = rs[r];
-      }
+    Pack<T> y[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) y[r][i] = v[r][i];
+    if (!last) load(row0 + R * steps.teams);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long row = row0 + r * steps.teams;
+      if (last && row >= rows) continue;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        at.store(y[r][i], (T*)y_.p + row * y_.stride, i);
     }
-  }
+  };
+  load(steps.start + steps.mine);
+  at.load_param(gain, w, 1.f);
+  at.load_param(shift, b, 0.f);
+  long first = steps.start;
+  wait_loads();
+  for (; steps.full(first, rows); first += R * steps.teams)
+    step(first + steps.mine, false);
+  if (first < rows) step(first + steps.mine, true);
 }
 
 // The backward pass of the same teams; part[block] = [2][cols], the
 // workgroup's column sums.  SUMS: dw and db are asked for.
 template <typename T, int THREADS, int TEAM, int NV, int R, bool EXACT,
-          bool SUMS>
+          bool SUMS, bool TINY>
 __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
     RowsIn dy_, RowsIn x_, const float* __restrict__ w,
     const float* __restrict__ mean, const float* __restrict__ rstd,
     RowsOut dx_, float* __restrict__ part, long rows, int cols) {
-  constexpr int N = Pack<T>::N, TEAMS = THREADS / TEAM, E = NV * N;
+  constexpr int N = Pack<T>::N, E = NV * N;
   __shared__ float tmp[4 * R * (THREADS / WAVE)];
   TeamSum<TEAM, 2 * R> sum{tmp, 0};
-  const Slots<T, TEAM, NV> at(cols);
+  const Slots<T, TEAM, NV, TINY> at(cols);
+  const Steps<THREADS, TEAM, R> steps;
   float gain[E], dw[E], db[E];
-  at.load_param(gain, w, 1.f);
-#pragma unroll
-  for (int k = 0; k < E; ++k) dw[k] = db[k] = 0.f;
-  const long teams = (long)gridDim.x * TEAMS;
   const float per = 1.f / cols;
-  for (long first = (long)blockIdx.x * TEAMS + (TEAM < THREADS
-                        ? (int)threadIdx.x / WAVE * (WAVE / TEAM) : 0);
-       first < rows; first += teams * R) {
-    const long row0 =
-        first + (TEAM < WAVE ? (threadIdx.x & (WAVE - 1)) / TEAM : 0);
-    Pack<T> vx[R][NV], vg[R][NV];
-    float mu[R], rs[R];
+  Pack<T> vx[R][NV], vg[R][NV];
+  float mu[R], rs[R];
+  auto load = [&](long row0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long row = row0 + r * teams;
-      const T* x = (const T*)x_.p + row * x_.stride;
-      const T* g = (const T*)dy_.p + row * dy_.stride;
-      mu[r] = rs[r] = 0.f;
-      if (row < rows) {
-        mu[r] = mean[row];
-        rs[r] = rstd[row];
-      }
+      const long row = min(row0 + r * steps.teams, rows - 1);
+      mu[r] = mean[row];
+      rs[r] = rstd[row];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        vx[r][i].fill(0.f);
-        vg[r][i].fill(0.f);
-        if (row < rows && at.has(i)) {
-          at.load(vx[r][i], x, i);
-          at.load(vg[r][i], g, i);
-        }
+        at.load(vx[r][i], (const T*)x_.p + row * x_.stride, i);
+        at.load(vg[r][i], (const T*)dy_.p + row * dy_.stride, i);
       }
     }
+  };
+  auto step = [&](long row0, bool last) {
     float s[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      if (last && row0 + r * steps.teams >= rows) {
+        mu[r] = rs[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          vx[r][i].fill(0.f);
+          vg[r][i].fill(0.f);
+        }
+      }
       s[2 * r] = s[2 * r + 1] = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        float e[N], g[N];
+        float e[N], g[N], s1 = 0.f, s2 = 0.f;
         vx[r][i].get(e);
         vg[r][i].get(g);
 #pragma unroll
@@ -392,19 +450,22 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
             db[i * N + k] += g[k];
           }
           float d = g[k] * gain[i * N + k];
-          if (!EXACT) d = at.template own<EXACT>(i, k) ? d : 0.f;
-          s[2 * r] += d;
-          s[2 * r + 1] = fmaf(d, h, s[2 * r + 1]);
+          if (!EXACT) d = at.own(i, k) ? d : 0.f;
+          s1 += d;
+          s2 = fmaf(d, h, s2);
         }
+        s[2 * r] += at.has(i) ? s1 : 0.f;
+        s[2 * r + 1] += at.has(i) ? s2 : 0.f;
       }
     }
-    if (!dx_.p) continue;
+    if (!dx_.p) {
+      if (!last) load(row0 + R * steps.teams);
+      return;
+    }
     sum(s);
+    Pack<T> out[R][NV];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long row = row0 + r * teams;
-      if (row >= rows) continue;
-      T* dx = (T*)dx_.p + row * dx_.stride;
       const float s1 = s[2 * r] * per, s2 = s[2 * r + 1] * per;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -418,11 +479,28 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
           const float h = (e[k] - mu[r]) * rs[r];
           g[k] = rs[r] * (fmaf(g[k], gain[i * N + k], -s1) - h * s2);
         }
-        vg[r][i].set(g);
-        if (at.has(i)) at.store(vg[r][i], dx, i);
+        out[r][i].set(g);
       }
     }
-  }
+    if (!last) load(row0 + R * steps.teams);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long row = row0 + r * steps.teams;
+      if (last && row >= rows) continue;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        at.store(out[r][i], (T*)dx_.p + row * dx_.stride, i);
+    }
+  };
+  load(steps.start + steps.mine);
+  at.load_param(gain, w, 1.f);
+#pragma unroll
+  for (int k = 0; k < E; ++k) dw[k] = db[k] = 0.f;
+  long first = steps.start;
+  wait_loads();
+  for (; steps.full(first, rows); first += R * steps.teams)
+    step(first + steps.mine, false);
+  if (first < rows) step(first + steps.mine, true);
   if (!SUMS) return;
   // the workgroup's sums: over the teams of a wave, then over the waves
   float* out = part + (long)blockIdx.x * 2 * cols;
@@ -459,7 +537,7 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      if (at.template own<false>(i, k)) {
+      if (at.own(i, k)) {
         out[at.at(i) + k] = dw[i * N + k];
         out[cols + at.at(i) + k] = db[i * N + k];
       }
@@ -477,25 +555,25 @@ static unsigned row_grid(long rows) {
 #define LN_TEAMS(cols, F)                                                    \
   do {                                                                       \
     if (cols <= 32) {                                                        \
-      F(256, 4, 8, 4);                                                       \
+      F(256, 4, 8, LN_RA);                                                   \
     } else if (cols <= 64) {                                                 \
-      F(256, 4, 16, 2);                                                      \
+      F(256, 8, 8, LN_RA);                                                   \
     } else if (cols <= 128) {                                                \
-      F(256, 16, 8, 4);                                                      \
+      F(256, 16, 8, LN_RA);                                                  \
     } else if (cols <= 256) {                                                \
-      F(256, 16, 16, 2);                                                     \
+      F(256, 32, 8, LN_RA);                                                  \
     } else if (cols <= 512) {                                                \
-      F(256, 64, 8, 4);                                                      \
+      F(256, 64, 8, LN_RA);                                                  \
     } else if (cols <= 1024) {                                               \
-      F(256, 64, 16, 2);                                                     \
+      F(128, 128, 8, LN_RB);                                                 \
     } else if (cols <= 2048) {                                               \
-      F(256, 256, 8, 4);                                                     \
+      F(256, 256, 8, LN_RB);                                                 \
     } else if (cols <= 4096) {                                               \
-      F(256, 256, 16, 2);                                                    \
+      F(512, 512, 8, LN_RB);                                                 \
     } else if (cols <= 8192) {                                               \
-      F(1024, 1024, 8, 2);                                                   \
+      F(1024, 1024, 8, LN_RB);                                               \
     } else {                                                                 \
-      F(1024, 1024, 16, 1);                                                  \
+      F(1024, 1024, 16, LN_RC);                                              \
     }                                                                        \
   } while (0)
 
@@ -516,17 +594,21 @@ static void ln_fwd_run(RowsIn x, RowsOut y, const float* w, const float* b,
     return;
   }
   const bool exact = cols % N == 0;
-#define RUN2(THREADS, TEAM, E, R, EXACT)                                     \
+#define RUN2(THREADS, TEAM, E, R, EXACT, TINY)                               \
   hipLaunchKernelGGL(                                                        \
-      HIP_KERNEL_NAME(ln_fwd_team_k<T, THREADS, TEAM, E / N, R, EXACT>),     \
-      dim3(team_grid(rows, THREADS / TEAM, R, 2048 * 256 / THREADS)),        \
+      HIP_KERNEL_NAME(                                                       \
+          ln_fwd_team_k<T, THREADS, TEAM, E / N, R, EXACT, TINY>),           \
+      dim3(team_grid(rows, THREADS / TEAM, R, LN_FB * 256 / THREADS)),        \
       dim3(THREADS), 0, s, x, y, w, b, mean, rstd, rows, cols, eps)
 #define RUN(THREADS, TEAM, E, R)                                             \
   if (exact)                                                                 \
-    RUN2(THREADS, TEAM, E, R, true);                                         \
+    RUN2(THREADS, TEAM, E, R, true, false);                                  \
   else                                                                       \
-    RUN2(THREADS, TEAM, E, R, false)
-  LN_TEAMS(cols, RUN);
+    RUN2(THREADS, TEAM, E, R, false, false)
+  if (cols < N)
+    RUN2(256, 4, 8, LN_RA, false, true);
+  else
+    LN_TEAMS(cols, RUN);
 #undef RUN
 #undef RUN2
 }
@@ -581,20 +663,25 @@ static void ln_bwd_run(RowsIn dy, RowsIn x, const float* w,
   }
   const unsigned grid = (unsigned)ln_parts(rows, cols);
   const bool exact = cols % N == 0;
-#define RUN2(THREADS, TEAM, E, R, EXACT, SUMS)                               \
+#define RUN2(THREADS, TEAM, E, R, EXACT, SUMS, TINY)                         \
   hipLaunchKernelGGL(                                                        \
       HIP_KERNEL_NAME(                                                       \
-          ln_bwd_team_k<T, THREADS, TEAM, E / N, R, EXACT, SUMS>),           \
+          ln_bwd_team_k<T, THREADS, TEAM, E / N, R, EXACT, SUMS, TINY>),     \
       dim3(grid), dim3(THREADS), 0, s, dy, x, w, mean, rstd, dx, part, rows, \
       cols)
 #define RUN(THREADS, TEAM, E, R)                                             \
   if (exact && sums)                                                         \
-    RUN2(THREADS, TEAM, E, R, true, true);                                   \
+    RUN2(THREADS, TEAM, E, R, true, true, false);                            \
   else if (sums)                                                             \
-    RUN2(THREADS, TEAM, E, R, false, true);                                  \
+    RUN2(THREADS, TEAM, E, R, false, true, false);                           \
   else                                                                       \
-    RUN2(THREADS, TEAM, E, R, false, false)
-  LN_TEAMS(cols, RUN);
+    RUN2(THREADS, TEAM, E, R, false, false, false)
+  if (cols < N && sums)
+    RUN2(256, 4, 8, LN_RA, false, true, true);
+  else if (cols < N)
+    RUN2(256, 4, 8, LN_RA, false, false, true);
+  else
+    LN_TEAMS(cols, RUN);
 #undef RUN
 #undef RUN2
 }

@@ -38,6 +38,21 @@ __device__ __forceinline__ V wave_join(V v, F f) {
 __device__ __forceinline__ float wave_sum(float v) {
   return wave_join(v, [](float a, float b) { return a + b; });
 }
+// (in the last lane alone)
+__device__ __forceinline__ float wave_sum_last(float v) {
+#define ROW_STEP(CTRL, ROWS)                                                 \
+  v += __builtin_bit_cast(                                                   \
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),      \
+                                         CTRL, ROWS, 0xf, false))
+  ROW_STEP(0x111, 0xf);    // from the lane 1, 2, 4, 8 before in the row of 16
+  ROW_STEP(0x112, 0xf);
+  ROW_STEP(0x114, 0xf);
+  ROW_STEP(0x118, 0xf);
+  ROW_STEP(0x142, 0xa);    // the rows' last lanes to the next rows
+  ROW_STEP(0x143, 0xc);
+#undef ROW_STEP
+  return v;
+}
 __device__ __forceinline__ float wave_max(float v) {
   return wave_join(v, [](float a, float b) { return fmaxf(a, b); });
 }
