@@ -10,17 +10,8 @@
 #include "rows.h"
 
 #define LN_THREADS 256
-// rows of partial column sums that a backward pass leaves to be joined
+// partial column sums of long rows that a backward pass leaves to be joined
 #define LN_PARTS 256
-// workgroups of 256 threads that a backward pass of teams has at most
-#define LN_BLOCKS 768
-#ifndef LN_RA
-#define LN_RA 2
-#define LN_RB 2
-#define LN_RC 1
-#define LN_FB 2048
-#define LN_ONCE 0
-#endif
 
 // one workgroup to a row; the row is read three times, from the caches
 // after the first
@@ -83,29 +74,44 @@ __global__ __launch_bounds__(LN_THREADS) void ln_bwd_k(
 }
 
 // column sums of dy xh and dy over this workgroup's rows: one thread to a
-// column, part[blockIdx.y] = [2][cols]
+// pack of columns (the last one ends with the row), part[blockIdx.y] =
+// [2][cols]
 template <typename T>
 __global__ __launch_bounds__(LN_THREADS) void ln_cols_k(
     RowsIn dy_, RowsIn x_, const float* __restrict__ mean,
     const float* __restrict__ rstd, float* __restrict__ part, long rows,
     int cols) {
-  const int j = blockIdx.x * LN_THREADS + threadIdx.x;
-  if (j >= cols) return;
+  constexpr int N = Pack<T>::N;
+  const int own = (blockIdx.x * LN_THREADS + threadIdx.x) * N;
+  if (own >= cols) return;
+  const int j = min(own, cols - N);
   const long per = (rows + gridDim.y - 1) / gridDim.y;
-  const long lo = blockIdx.y * per;
-  const long hi = lo + per < rows ? lo + per : rows;
-  float sw = 0.f, sb = 0.f;
+  const long lo = blockIdx.y * per, hi = min(lo + per, rows);
+  float sw[N], sb[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) sw[k] = sb[k] = 0.f;
+#pragma unroll 4
   for (long row = lo; row < hi; ++row) {
-    const float g = (float)((const T*)dy_.p)[row * dy_.stride + j];
-    const float h =
-        ((float)((const T*)x_.p)[row * x_.stride + j] - mean[row]) *
-        rstd[row];
-    sw += g * h;
-    sb += g;
+    Pack<T> vg, vx;
+    float g[N], e[N];
+    vg.load((const T*)dy_.p + row * dy_.stride + j);
+    vx.load((const T*)x_.p + row * x_.stride + j);
+    vg.get(g);
+    vx.get(e);
+    const float mu = mean[row], rs = rstd[row];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      sw[k] = fmaf(g[k], (e[k] - mu) * rs, sw[k]);
+      sb[k] += g[k];
+    }
   }
   float* out = part + (long)blockIdx.y * 2 * cols;
-  out[j] = sw;
-  out[cols + j] = sb;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (j + k >= own) {
+      out[j + k] = sw[k];
+      out[cols + j + k] = sb[k];
+    }
 }
 
 // The partial sums [parts][2][cols] joined, always in the same order: 32 of
@@ -144,7 +150,7 @@ __global__ __launch_bounds__(LN_THREADS) void ln_join_k(
 
 // the team's sums of R values each, in all its lanes; `tmp`: [2][R][waves],
 // used in turn so that one barrier does for a call
-template <int TEAM, int R>
+template <int THREADS, int TEAM, int R>
 struct TeamSum {
   float* tmp;
   int turn;
@@ -166,19 +172,19 @@ struct TeamSum {
     } else {
       // a wave's sum comes to its last lane; the waves' are joined by a lane
       // to each
-      constexpr int WAVES = TEAM / WAVE;
-      float* t = tmp + turn * R * WAVES;
+      constexpr int WAVES = TEAM / WAVE, ALL = THREADS / WAVE;
+      float* t = tmp + turn * R * ALL;
       turn ^= 1;
-      const int lane = threadIdx.x & (WAVE - 1);
+      const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         const float w = wave_sum_last(v[i]);
-        if (lane == WAVE - 1) t[i * WAVES + threadIdx.x / WAVE] = w;
+        if (lane == WAVE - 1) t[i * ALL + wave] = w;
       }
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        v[i] = t[i * WAVES + lane % WAVES];
+        v[i] = t[i * ALL + wave / WAVES * WAVES + lane % WAVES];
         v[i] += other_lane<0xb1>(v[i]);
         if (WAVES > 2) v[i] += other_lane<0x4e>(v[i]);
         if (WAVES > 4) v[i] += other_lane<0x141>(v[i]);
@@ -208,7 +214,7 @@ struct Slots {
   int lane, cols, packs;
 
   __device__ __forceinline__ Slots(int cols_) {
-    lane = TEAM <= WAVE ? threadIdx.x % TEAM : threadIdx.x;
+    lane = threadIdx.x % TEAM;
     cols = cols_;
     packs = (cols + N - 1) / N;
   }
@@ -221,8 +227,13 @@ struct Slots {
   }
   // whether element k of pack i is this pack's own
   __device__ __forceinline__ bool own(int i, int k) const {
-    const int j = (i * TEAM + lane) * N;
-    return has(i) && at(i) + k >= j && at(i) + k < cols;
+    return column(lane, i, k) >= 0;
+  }
+  // the column of element k of a lane's pack i, -1 if it is another's
+  __device__ __forceinline__ int column(int of, int i, int k) const {
+    const int j = (i * TEAM + of) * N;
+    const int c = (TINY ? 0 : min(j, cols - N)) + k;
+    return i * TEAM + of < packs && c >= j && c < cols ? c : -1;
   }
   __device__ __forceinline__ void load(Pack<T>& v, const T* row, int i) const {
     if (TINY) {
@@ -257,26 +268,24 @@ struct Slots {
   }
 };
 
-// The rows of a team: from `start`, `step` apart R at a time.  All lanes of
-// a wave (a workgroup, where it is the team) make the same number of steps.
-template <int THREADS, int TEAM, int R>
+// The rows of a team: those of a workgroup's teams from `start`, and `teams`
+// apart.  All lanes of a workgroup make the same number of steps.
+template <int THREADS, int TEAM>
 struct Steps {
   long start, teams;
-  int mine;        // this lane's team among those of its wave
+  int mine;        // this lane's team among those of its workgroup
 
   __device__ __forceinline__ Steps() {
     constexpr int TEAMS = THREADS / TEAM;
     teams = (long)gridDim.x * TEAMS;
     start = (long)blockIdx.x * TEAMS;
-    if (TEAM < THREADS)
-      start += __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) *
-               (TEAM < WAVE ? WAVE / TEAM : 1);
-    mine = TEAM < WAVE ? (threadIdx.x & (WAVE - 1)) / TEAM : 0;
+    // (the same number for a wave, where it is one)
+    mine = TEAM < WAVE ? (int)threadIdx.x / TEAM
+                       : __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM);
   }
   // whether all rows of the step from `first` exist
   __device__ __forceinline__ bool full(long first, long rows) const {
-    return first + (R - 1) * teams + (TEAM < WAVE ? WAVE / TEAM - 1 : 0) <
-           rows;
+    return first + THREADS / TEAM - 1 < rows;
   }
 };
 
@@ -291,294 +300,250 @@ __device__ __forceinline__ void wait_loads() {
 // operations are waited for in their order, and what waits for a load would
 // otherwise wait for stores to reach memory.  For the same reason nothing
 // after those loads is on a condition; the last step is apart.
-template <typename T, int THREADS, int TEAM, int NV, int R, bool EXACT,
-          bool TINY>
+template <typename T, int THREADS, int TEAM, int NV, bool EXACT, bool TINY>
 __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
     RowsIn x_, RowsOut y_, const float* __restrict__ w,
     const float* __restrict__ b, float* __restrict__ mean,
     float* __restrict__ rstd, long rows, int cols, float eps) {
   constexpr int N = Pack<T>::N;
-  __shared__ float tmp[2 * R * (THREADS / WAVE)];
-  TeamSum<TEAM, R> sum{tmp, 0};
+  __shared__ float tmp[2 * (THREADS / WAVE)];
+  TeamSum<THREADS, TEAM, 1> sum{tmp, 0};
   const Slots<T, TEAM, NV, TINY> at(cols);
-  const Steps<THREADS, TEAM, R> steps;
+  const Steps<THREADS, TEAM> steps;
   float gain[NV * N], shift[NV * N];
   const float per = 1.f / cols;
-  Pack<T> v[R][NV];
-  auto load = [&](long row0) {
+  Pack<T> v[NV];
+  auto load = [&](long row) {
+    row = min(row, rows - 1);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long row = min(row0 + r * steps.teams, rows - 1);
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        at.load(v[r][i], (const T*)x_.p + row * x_.stride, i);
-    }
+    for (int i = 0; i < NV; ++i)
+      at.load(v[i], (const T*)x_.p + row * x_.stride, i);
   };
-  auto step = [&](long row0, bool last) {
-    float mu[R], rs[R];
+  auto step = [&](long row, bool last) {
+    float mu = 0.f, rs = 0.f;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      mu[r] = 0.f;
+    for (int i = 0; i < NV; ++i) {
+      float e[N], q = 0.f;
+      v[i].get(e);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float e[N], q = 0.f;
-        v[r][i].get(e);
+      for (int k = 0; k < N; ++k) q += EXACT || at.own(i, k) ? e[k] : 0.f;
+      mu += at.has(i) ? q : 0.f;
+    }
+    sum(&mu);
+    mu *= per;
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-          q += EXACT || at.own(i, k) ? e[k] : 0.f;
-        mu[r] += at.has(i) ? q : 0.f;
+    for (int i = 0; i < NV; ++i) {
+      float e[N], q = 0.f;
+      v[i].forget();
+      v[i].get(e);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        float d = e[k] - mu;
+        if (!EXACT) d = at.own(i, k) ? d : 0.f;
+        q = fmaf(d, d, q);
       }
+      rs += at.has(i) ? q : 0.f;
     }
-    sum(mu);
+    sum(&rs);
+    rs = inv_sqrt(fmaf(rs, per, eps));
+    if (at.lane == 0 && mean && row < rows) mean[row] = mu;
+    if (at.lane == 0 && rstd && row < rows) rstd[row] = rs;
+    Pack<T> y[NV];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      mu[r] *= per;
-      rs[r] = 0.f;
+    for (int i = 0; i < NV; ++i) {
+      float e[N];
+      v[i].forget();
+      v[i].get(e);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float e[N], q = 0.f;
-        v[r][i].forget();
-        v[r][i].get(e);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          float d = e[k] - mu[r];
-          if (!EXACT) d = at.own(i, k) ? d : 0.f;
-          q = fmaf(d, d, q);
-        }
-        rs[r] += at.has(i) ? q : 0.f;
-      }
+      for (int k = 0; k < N; ++k)
+        e[k] = fmaf((e[k] - mu) * rs, gain[i * N + k], shift[i * N + k]);
+      y[i].set(e);
     }
-    sum(rs);
+    if (!last) load(row + steps.teams);
+    if (last && row >= rows) return;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long row = row0 + r * steps.teams;
-      rs[r] = inv_sqrt(fmaf(rs[r], per, eps));
-      if (at.lane == 0 && mean && row < rows) mean[row] = mu[r];
-      if (at.lane == 0 && rstd && row < rows) rstd[row] = rs[r];
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float e[N];
-        v[r][i].forget();
-        v[r][i].get(e);
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-          e[k] = fmaf((e[k] - mu[r]) * rs[r], gain[i * N + k],
-                      shift[i * N + k]);
-        v[r][i].set(e);
-      }
-    Pack<T> y[R][NV];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) y[r][i] = v[r][i];
-    if (!last) load(row0 + R * steps.teams);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long row = row0 + r * steps.teams;
-      if (last && row >= rows) continue;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        at.store(y[r][i], (T*)y_.p + row * y_.stride, i);
-    }
+    for (int i = 0; i < NV; ++i)
+      at.store(y[i], (T*)y_.p + row * y_.stride, i);
   };
   load(steps.start + steps.mine);
   at.load_param(gain, w, 1.f);
   at.load_param(shift, b, 0.f);
-  long first = steps.start;
   wait_loads();
-  for (; steps.full(first, rows); first += R * steps.teams)
+  long first = steps.start;
+  for (; steps.full(first, rows); first += steps.teams)
     step(first + steps.mine, false);
   if (first < rows) step(first + steps.mine, true);
 }
 
 // The backward pass of the same teams; part[block] = [2][cols], the
-// workgroup's column sums.  SUMS: dw and db are asked for.
-template <typename T, int THREADS, int TEAM, int NV, int R, bool EXACT,
-          bool SUMS, bool TINY>
+// workgroup's column sums.  SUMS: dw or db is asked for, DX: dx is.
+template <typename T, int THREADS, int TEAM, int NV, bool EXACT, bool SUMS,
+          bool DX, bool TINY>
 __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
     RowsIn dy_, RowsIn x_, const float* __restrict__ w,
     const float* __restrict__ mean, const float* __restrict__ rstd,
     RowsOut dx_, float* __restrict__ part, long rows, int cols) {
   constexpr int N = Pack<T>::N, E = NV * N;
-  __shared__ float tmp[4 * R * (THREADS / WAVE)];
-  TeamSum<TEAM, 2 * R> sum{tmp, 0};
+  __shared__ float tmp[4 * (THREADS / WAVE)];
+  TeamSum<THREADS, TEAM, 2> sum{tmp, 0};
   const Slots<T, TEAM, NV, TINY> at(cols);
-  const Steps<THREADS, TEAM, R> steps;
+  const Steps<THREADS, TEAM> steps;
   float gain[E], dw[E], db[E];
   const float per = 1.f / cols;
-  Pack<T> vx[R][NV], vg[R][NV];
-  float mu[R], rs[R];
-  auto load = [&](long row0) {
+  Pack<T> vx[NV], vg[NV];
+  float mu, rs;
+  auto load = [&](long row) {
+    row = min(row, rows - 1);
+    mu = mean[row];
+    rs = rstd[row];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long row = min(row0 + r * steps.teams, rows - 1);
-      mu[r] = mean[row];
-      rs[r] = rstd[row];
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        at.load(vx[r][i], (const T*)x_.p + row * x_.stride, i);
-        at.load(vg[r][i], (const T*)dy_.p + row * dy_.stride, i);
-      }
+    for (int i = 0; i < NV; ++i) {
+      at.load(vx[i], (const T*)x_.p + row * x_.stride, i);
+      at.load(vg[i], (const T*)dy_.p + row * dy_.stride, i);
     }
   };
-  auto step = [&](long row0, bool last) {
-    float s[2 * R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (last && row0 + r * steps.teams >= rows) {
-        mu[r] = rs[r] = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          vx[r][i].fill(0.f);
-          vg[r][i].fill(0.f);
-        }
-      }
-      s[2 * r] = s[2 * r + 1] = 0.f;
+  auto step = [&](long row, bool last) {
+    if (last && row >= rows) {
+      mu = rs = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        float e[N], g[N], s1 = 0.f, s2 = 0.f;
-        vx[r][i].get(e);
-        vg[r][i].get(g);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const float h = (e[k] - mu[r]) * rs[r];
-          if (SUMS) {
-            dw[i * N + k] = fmaf(g[k], h, dw[i * N + k]);
-            db[i * N + k] += g[k];
-          }
-          float d = g[k] * gain[i * N + k];
-          if (!EXACT) d = at.own(i, k) ? d : 0.f;
-          s1 += d;
-          s2 = fmaf(d, h, s2);
-        }
-        s[2 * r] += at.has(i) ? s1 : 0.f;
-        s[2 * r + 1] += at.has(i) ? s2 : 0.f;
+        vx[i].fill(0.f);
+        vg[i].fill(0.f);
       }
     }
-    if (!dx_.p) {
-      if (!last) load(row0 + R * steps.teams);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float e[N], g[N], s1 = 0.f, s2 = 0.f;
+      vx[i].get(e);
+      vg[i].get(g);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float h = (e[k] - mu) * rs;
+        if (SUMS) {
+          dw[i * N + k] = fmaf(g[k], h, dw[i * N + k]);
+          db[i * N + k] += g[k];
+        }
+        float d = g[k] * gain[i * N + k];
+        if (!EXACT) d = at.own(i, k) ? d : 0.f;
+        s1 += d;
+        s2 = fmaf(d, h, s2);
+      }
+      s[0] += at.has(i) ? s1 : 0.f;
+      s[1] += at.has(i) ? s2 : 0.f;
+    }
+    if (!DX) {
+      if (!last) load(row + steps.teams);
       return;
     }
     sum(s);
-    Pack<T> out[R][NV];
+    const float s1 = s[0] * per, s2 = s[1] * per;
+    Pack<T> out[NV];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float s1 = s[2 * r] * per, s2 = s[2 * r + 1] * per;
+    for (int i = 0; i < NV; ++i) {
+      float e[N], g[N];
+      vx[i].forget();
+      vg[i].forget();
+      vx[i].get(e);
+      vg[i].get(g);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float e[N], g[N];
-        vx[r][i].forget();
-        vg[r][i].forget();
-        vx[r][i].get(e);
-        vg[r][i].get(g);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const float h = (e[k] - mu[r]) * rs[r];
-          g[k] = rs[r] * (fmaf(g[k], gain[i * N + k], -s1) - h * s2);
-        }
-        out[r][i].set(g);
+      for (int k = 0; k < N; ++k) {
+        const float h = (e[k] - mu) * rs;
+        g[k] = rs * (fmaf(g[k], gain[i * N + k], -s1) - h * s2);
       }
+      out[i].set(g);
     }
-    if (!last) load(row0 + R * steps.teams);
+    if (!last) load(row + steps.teams);
+    if (last && row >= rows) return;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long row = row0 + r * steps.teams;
-      if (last && row >= rows) continue;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        at.store(out[r][i], (T*)dx_.p + row * dx_.stride, i);
-    }
+    for (int i = 0; i < NV; ++i)
+      at.store(out[i], (T*)dx_.p + row * dx_.stride, i);
   };
   load(steps.start + steps.mine);
   at.load_param(gain, w, 1.f);
 #pragma unroll
   for (int k = 0; k < E; ++k) dw[k] = db[k] = 0.f;
-  long first = steps.start;
   wait_loads();
-  for (; steps.full(first, rows); first += R * steps.teams)
+  long first = steps.start;
+  for (; steps.full(first, rows); first += steps.teams)
     step(first + steps.mine, false);
   if (first < rows) step(first + steps.mine, true);
   if (!SUMS) return;
-  // the workgroup's sums: over the teams of a wave, then over the waves
-  float* out = part + (long)blockIdx.x * 2 * cols;
-  if constexpr (TEAM < THREADS) {
-    __shared__ float all[2 * E * TEAM];
+  // the workgroup's sums: over the teams of a wave, then over the waves that
+  // have the same columns
+  constexpr int LANES = TEAM < WAVE ? TEAM : WAVE;     // of a wave
+  constexpr int SETS = TEAM < WAVE ? THREADS / WAVE : THREADS / TEAM;
+  __shared__ float all[SETS][E * TEAM];
+  const int set = TEAM < WAVE ? threadIdx.x / WAVE : threadIdx.x / TEAM;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
 #pragma unroll
     for (int k = 0; k < E; ++k) {
+      float d = half ? db[k] : dw[k];
 #pragma unroll
-      for (int off = TEAM; off < WAVE; off *= 2) {
-        dw[k] += __shfl_xor(dw[k], off);
-        db[k] += __shfl_xor(db[k], off);
-      }
+      for (int off = LANES; off < WAVE; off *= 2) d += __shfl_xor(d, off);
+      if (TEAM >= WAVE || (threadIdx.x & (WAVE - 1)) < TEAM)
+        all[set][k * TEAM + at.lane] = d;
     }
-    const int lane = threadIdx.x & (WAVE - 1);
-    for (int v = 0; v < THREADS / WAVE; ++v) {
-      if ((int)threadIdx.x / WAVE == v && lane < TEAM) {
+    __syncthreads();
+    float* out = part + (2l * blockIdx.x + half) * cols;
+    for (int a = threadIdx.x; a < E * TEAM; a += THREADS) {
+      const int c = at.column(a % TEAM, a / TEAM / N, a / TEAM % N);
+      if (c < 0) continue;
+      float d = all[0][a];
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-          const int a = k * TEAM + lane;
-          all[a] = v ? all[a] + dw[k] : dw[k];
-          all[E * TEAM + a] = v ? all[E * TEAM + a] + db[k] : db[k];
-        }
-      }
-      __syncthreads();
+      for (int v = 1; v < SETS; ++v) d += all[v][a];
+      out[c] = d;
     }
-    if ((int)threadIdx.x >= TEAM) return;
-#pragma unroll
-    for (int k = 0; k < E; ++k) {
-      dw[k] = all[k * TEAM + lane];
-      db[k] = all[E * TEAM + k * TEAM + lane];
-    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (at.own(i, k)) {
-        out[at.at(i) + k] = dw[i * N + k];
-        out[cols + at.at(i) + k] = db[i * N + k];
-      }
 }
 
 static unsigned row_grid(long rows) {
   return (unsigned)(rows < 65536 ? rows : 65536);
 }
 
-// the elements of a row that a team of lanes holds at most: 8 or 16 each
-#define LN_MOST 16384
+// Rows of as many elements are held by teams: of 8 a lane up to 8192, then
+// of 16 and 32 (forward; backward 16, or 32 without the column sums).
+#define LN_MOST 32768
+#define LN_MOST_SUMS 16384
+// Workgroups at most: 2048 of 256 threads forward (16384 x 4096 bf16 in 51
+// us, with 4096 of them 71, 8192 87).  Backward 256 of 1024 threads, one to a
+// compute unit, so that few column sums are left to be joined (84 us; 512 of
+// them, in turns, 90; 128 118).
+#define LN_FORWARD 2048
+#define LN_BACKWARD 256
 
-// F(threads, team, elements of a lane, rows at a time) of the first team
-// that holds a row
+// F(threads, team, elements of a lane) of the first team that holds a row
 #define LN_TEAMS(cols, F)                                                    \
   do {                                                                       \
     if (cols <= 32) {                                                        \
-      F(256, 4, 8, LN_RA);                                                   \
+      F(256, 4, 8);                                                          \
     } else if (cols <= 64) {                                                 \
-      F(256, 8, 8, LN_RA);                                                   \
+      F(256, 8, 8);                                                          \
     } else if (cols <= 128) {                                                \
-      F(256, 16, 8, LN_RA);                                                  \
+      F(256, 16, 8);                                                         \
     } else if (cols <= 256) {                                                \
-      F(256, 32, 8, LN_RA);                                                  \
+      F(256, 32, 8);                                                         \
     } else if (cols <= 512) {                                                \
-      F(256, 64, 8, LN_RA);                                                  \
+      F(256, 64, 8);                                                         \
     } else if (cols <= 1024) {                                               \
-      F(128, 128, 8, LN_RB);                                                 \
+      F(128, 128, 8);                                                        \
     } else if (cols <= 2048) {                                               \
-      F(256, 256, 8, LN_RB);                                                 \
+      F(256, 256, 8);                                                        \
     } else if (cols <= 4096) {                                               \
-      F(512, 512, 8, LN_RB);                                                 \
+      F(512, 512, 8);                                                        \
     } else if (cols <= 8192) {                                               \
-      F(1024, 1024, 8, LN_RB);                                               \
+      F(1024, 1024, 8);                                                      \
+    } else if (cols <= 16384) {                                              \
+      F(1024, 1024, 16);                                                     \
     } else {                                                                 \
-      F(1024, 1024, 16, LN_RC);                                              \
+      F(1024, 1024, 32);                                                     \
     }                                                                        \
   } while (0)
 
-static unsigned team_grid(long rows, int teams, int at_once, long most) {
-  const long n = (rows + (long)teams * at_once - 1) / ((long)teams * at_once);
+static unsigned team_grid(long rows, int teams, long most) {
+  const long n = (rows + teams - 1) / teams;
   return (unsigned)(n < most ? n : most);
 }
 
@@ -593,20 +558,18 @@ static void ln_fwd_run(RowsIn x, RowsOut y, const float* w, const float* b,
                        cols, eps);
     return;
   }
-  const bool exact = cols % N == 0;
-#define RUN2(THREADS, TEAM, E, R, EXACT, TINY)                               \
+#define RUN2(THREADS, TEAM, E, EXACT, TINY)                                  \
   hipLaunchKernelGGL(                                                        \
-      HIP_KERNEL_NAME(                                                       \
-          ln_fwd_team_k<T, THREADS, TEAM, E / N, R, EXACT, TINY>),           \
-      dim3(team_grid(rows, THREADS / TEAM, R, LN_FB * 256 / THREADS)),        \
+      HIP_KERNEL_NAME(ln_fwd_team_k<T, THREADS, TEAM, E / N, EXACT, TINY>),  \
+      dim3(team_grid(rows, THREADS / TEAM, LN_FORWARD * 256 / THREADS)),     \
       dim3(THREADS), 0, s, x, y, w, b, mean, rstd, rows, cols, eps)
-#define RUN(THREADS, TEAM, E, R)                                             \
-  if (exact)                                                                 \
-    RUN2(THREADS, TEAM, E, R, true, false);                                  \
+#define RUN(THREADS, TEAM, E)                                                \
+  if (cols % N == 0)                                                         \
+    RUN2(THREADS, TEAM, E, true, false);                                     \
   else                                                                       \
-    RUN2(THREADS, TEAM, E, R, false, false)
+    RUN2(THREADS, TEAM, E, false, false)
   if (cols < N)
-    RUN2(256, 4, 8, LN_RA, false, true);
+    RUN2(256, 4, 8, false, true);
   else
     LN_TEAMS(cols, RUN);
 #undef RUN
@@ -623,12 +586,11 @@ void layer_norm_fwd_launch(int type, RowsIn x, RowsOut y, const float* w,
   HIP_CHECK_LAST();
 }
 
-// workgroups of a backward pass that leaves partial sums
+// workgroups of a backward pass, or partial sums that it leaves
 static long ln_parts(long rows, int cols) {
-  if (cols > LN_MOST) return rows < LN_PARTS ? rows : LN_PARTS;
+  if (cols > LN_MOST_SUMS) return rows < LN_PARTS ? rows : LN_PARTS;
   long n = 0;
-#define GRID(THREADS, TEAM, E, R)                                            \
-  n = team_grid(rows, THREADS / TEAM, R, LN_BLOCKS * 256 / THREADS)
+#define GRID(THREADS, TEAM, E) n = team_grid(rows, 1024 / TEAM, LN_BACKWARD)
   LN_TEAMS(cols, GRID);
 #undef GRID
   return n;
@@ -646,42 +608,51 @@ static void ln_bwd_run(RowsIn dy, RowsIn x, const float* w,
                        bool sums, float* part, long rows, int cols,
                        hipStream_t s) {
   constexpr int N = Pack<T>::N;
-  if (cols > LN_MOST) {
+  if (cols > LN_MOST_SUMS) {
     // the sums first: dx may be written over dy or x
-    if (sums)
-      hipLaunchKernelGGL(
-          HIP_KERNEL_NAME(ln_cols_k<T>),
-          dim3((cols + LN_THREADS - 1) / LN_THREADS,
-               (unsigned)ln_parts(rows, cols)),
-          dim3(LN_THREADS), 0, s, dy, x, mean, rstd, part, rows, cols);
-    HIP_CHECK_LAST();
-    if (dx.p)
+    if (sums) {
+      const int packs = (cols + N - 1) / N;
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(ln_cols_k<T>),
+                         dim3((packs + LN_THREADS - 1) / LN_THREADS,
+                              (unsigned)ln_parts(rows, cols)),
+                         dim3(LN_THREADS), 0, s, dy, x, mean, rstd, part,
+                         rows, cols);
+      HIP_CHECK_LAST();
+    }
+    if (!dx.p) return;
+    if (cols > LN_MOST) {
       hipLaunchKernelGGL(HIP_KERNEL_NAME(ln_bwd_k<T>), dim3(row_grid(rows)),
                          dim3(LN_THREADS), 0, s, dy, x, w, mean, rstd, dx,
                          rows, cols);
-    return;
+      return;
+    }
+    sums = false;
   }
-  const unsigned grid = (unsigned)ln_parts(rows, cols);
-  const bool exact = cols % N == 0;
-#define RUN2(THREADS, TEAM, E, R, EXACT, SUMS, TINY)                         \
+  const dim3 grid((unsigned)ln_parts(rows, cols));
+#define RUN2(TEAM, E, EXACT, SUMS, DX, TINY)                                 \
   hipLaunchKernelGGL(                                                        \
       HIP_KERNEL_NAME(                                                       \
-          ln_bwd_team_k<T, THREADS, TEAM, E / N, R, EXACT, SUMS, TINY>),     \
-      dim3(grid), dim3(THREADS), 0, s, dy, x, w, mean, rstd, dx, part, rows, \
-      cols)
-#define RUN(THREADS, TEAM, E, R)                                             \
-  if (exact && sums)                                                         \
-    RUN2(THREADS, TEAM, E, R, true, true, false);                            \
+          ln_bwd_team_k<T, 1024, TEAM, E / N, EXACT, SUMS, DX, TINY>),       \
+      grid, dim3(1024), 0, s, dy, x, w, mean, rstd, dx, part, rows, cols)
+#define RUN(THREADS, TEAM, E)                                                \
+  if constexpr (E == 32)                                                     \
+    RUN2(TEAM, E, false, false, true, false);                                \
+  else if (cols % N == 0 && sums && dx.p)                                    \
+    RUN2(TEAM, E, true, true, true, false);                                  \
+  else if (sums && dx.p)                                                     \
+    RUN2(TEAM, E, false, true, true, false);                                 \
   else if (sums)                                                             \
-    RUN2(THREADS, TEAM, E, R, false, true, false);                           \
+    RUN2(TEAM, E, false, true, false, false);                                \
   else                                                                       \
-    RUN2(THREADS, TEAM, E, R, false, false, false)
-  if (cols < N && sums)
-    RUN2(256, 4, 8, LN_RA, false, true, true);
-  else if (cols < N)
-    RUN2(256, 4, 8, LN_RA, false, false, true);
-  else
+    RUN2(TEAM, E, false, false, true, false)
+  if (cols >= N)
     LN_TEAMS(cols, RUN);
+  else if (sums && dx.p)
+    RUN2(4, 8, false, true, true, true);
+  else if (sums)
+    RUN2(4, 8, false, true, false, true);
+  else
+    RUN2(4, 8, false, false, true, true);
 #undef RUN
 #undef RUN2
 }
