@@ -306,6 +306,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
     const float* __restrict__ b, float* __restrict__ mean,
     float* __restrict__ rstd, long rows, int cols, float eps) {
   constexpr int N = Pack<T>::N;
+  constexpr bool AHEAD = NV < 8;       // (fp32 of 32 elements: no registers)
   __shared__ float tmp[2 * (THREADS / WAVE)];
   TeamSum<THREADS, TEAM, 1> sum{tmp, 0};
   const Slots<T, TEAM, NV, TINY> at(cols);
@@ -359,11 +360,12 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
         e[k] = fmaf((e[k] - mu) * rs, gain[i * N + k], shift[i * N + k]);
       y[i].set(e);
     }
-    if (!last) load(row + steps.teams);
+    if (AHEAD && !last) load(row + steps.teams);
     if (last && row >= rows) return;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       at.store(y[i], (T*)y_.p + row * y_.stride, i);
+    if (!AHEAD && !last) load(row + steps.teams);
   };
   load(steps.start + steps.mine);
   at.load_param(gain, w, 1.f);
@@ -384,6 +386,7 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
     const float* __restrict__ mean, const float* __restrict__ rstd,
     RowsOut dx_, float* __restrict__ part, long rows, int cols) {
   constexpr int N = Pack<T>::N, E = NV * N;
+  constexpr bool AHEAD = NV < 8;
   __shared__ float tmp[4 * (THREADS / WAVE)];
   TeamSum<THREADS, TEAM, 2> sum{tmp, 0};
   const Slots<T, TEAM, NV, TINY> at(cols);
@@ -453,11 +456,12 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
       }
       out[i].set(g);
     }
-    if (!last) load(row + steps.teams);
+    if (AHEAD && !last) load(row + steps.teams);
     if (last && row >= rows) return;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       at.store(out[i], (T*)dx_.p + row * dx_.stride, i);
+    if (!AHEAD && !last) load(row + steps.teams);
   };
   load(steps.start + steps.mine);
   at.load_param(gain, w, 1.f);
