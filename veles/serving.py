@@ -98,7 +98,9 @@ class InferenceEngine(object):
                                         dtype=out.devmem.dtype,
                                         pin_memory=True)
         self._out_pin.copy_(out.devmem)
-        return self._out_pin[:n].float().numpy()
+        # (a copy: .float() of an fp32 head is the pinned buffer itself,
+        # which the next batch overwrites)
+        return self._out_pin[:n].float().clone().numpy()
 
     def _run_numpy(self, x):
         self._in.map_invalidate()
