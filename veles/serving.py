@@ -13,6 +13,7 @@ launch-bound, exactly the regime graph replay removes.
     eng = InferenceEngine("snap.4.pickle.gz")      # auto device
     probs = eng.predict(batch_ndarray)             # [n, n_classes]
     labels = probs.argmax(1)
+    ans = eng.predict_top(batch_ndarray, 5)        # likeliest classes
 
     python -m veles.serving snap.pickle.gz --port 8080   # HTTP JSON
 """
@@ -49,6 +50,7 @@ class InferenceEngine(object):
         self.batch_size = batch_size or int(wf.loader.max_minibatch_size)
         self._in = wf.loader.minibatch_data
         self._graph = None
+        self._top_graphs = {}          # alternatives -> (graph, outputs)
         self._lock = threading.Lock()
 
     # -- core ---------------------------------------------------------------
@@ -56,7 +58,20 @@ class InferenceEngine(object):
         for f in self.forwards:
             f.run()
 
-    def _run_device(self, x):
+    def _forward_logits(self):
+        """The forward pass up to the logits: those of a softmax head, or
+        what another head gives."""
+        head = self.forwards[-1]
+        soft = hasattr(head, "logits_only")
+        if soft:
+            head.logits_only = True
+        try:
+            self._forward()
+        finally:
+            if soft:
+                head.logits_only = False
+
+    def _upload(self, x):
         import torch
         n = x.shape[0]
         dev = self._in.devmem
@@ -73,6 +88,11 @@ class InferenceEngine(object):
         dev[:n].copy_(self._pin[:n], non_blocking=True)
         if n < dev.shape[0]:
             dev[n:] = 0
+
+    def _run_device(self, x):
+        import torch
+        self._upload(x)
+        n = x.shape[0]
         if self._graph is None:
             # warm up once eagerly, then capture the forward chain
             self._forward()
@@ -131,6 +151,103 @@ class InferenceEngine(object):
 
     def predict_labels(self, x):
         return self.predict(x).reshape(x.shape[0], -1).argmax(axis=1)
+
+    # -- answers with their log probabilities --------------------------------
+    def _top_device(self, x, labels, top):
+        import torch
+        from veles.znicz_amd import ops
+        self._upload(x)
+        out = self.forwards[-1].output
+        if top not in self._top_graphs:
+            batch, dev = out.devmem.shape[0], out.devmem.device
+            outs = {
+                "labels": torch.full((batch,), -1, dtype=torch.int32,
+                                     device=dev),
+                "logprob": torch.empty(batch, device=dev),
+                "entropy": torch.empty(batch, device=dev),
+                "top": torch.empty(batch, top, dtype=torch.int32,
+                                   device=dev),
+                "top_logprob": torch.empty(batch, top, device=dev)}
+
+            def run():
+                self._forward_logits()
+                ops.token_logprobs(ops.as2d(out), outs["labels"],
+                                   outs["logprob"], outs["entropy"],
+                                   outs["top"], outs["top_logprob"])
+
+            run()                      # warm up, then capture as predict()
+            graph = None
+            try:
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    run()
+                graph = g
+            except Exception:          # eager, permanently
+                graph = None
+            self._top_graphs[top] = (graph, run, outs)
+        graph, run, outs = self._top_graphs[top]
+        given = numpy.full(outs["labels"].shape[0], -1, numpy.int32)
+        if labels is not None:
+            given[:len(labels)] = labels
+        outs["labels"].copy_(torch.from_numpy(given))
+        if graph is not None:
+            graph.replay()
+        else:
+            run()
+        out.touch_device()
+        n = x.shape[0]
+        return {k: v[:n].cpu().numpy() for k, v in outs.items()
+                if k != "labels"}
+
+    def _top_numpy(self, x, labels, top):
+        from veles.znicz_amd.distillation import numpy_logprobs
+        n = x.shape[0]
+        self._in.map_invalidate()
+        self._in.mem[:n] = x
+        self._in.mem[n:] = 0
+        self._forward_logits()
+        out = self.forwards[-1].output
+        out.map_read()
+        lp, ent, idx, top_lp = numpy_logprobs(
+            out.mem[:n].reshape(n, -1),
+            numpy.full(n, -1) if labels is None else labels, top)
+        return {"logprob": lp.astype(numpy.float32),
+                "entropy": ent.astype(numpy.float32), "top": idx,
+                "top_logprob": top_lp.astype(numpy.float32)}
+
+    def predict_top(self, x, top=5, labels=None):
+        """The likeliest classes of each sample with their log probabilities:
+        {"top": int32[n, top], "top_logprob": fp32[n, top], "entropy":
+        fp32[n]} and, for given ``labels``, "logprob": fp32[n].  ``top`` is 1
+        to 128; places beyond the number of classes hold -1 and minus
+        infinity."""
+        x = numpy.asarray(x, numpy.float32)
+        if x.shape[1:] != tuple(self._in.shape[1:]):
+            raise ValueError("sample shape %s != model input %s" %
+                             (x.shape[1:], tuple(self._in.shape[1:])))
+        top = int(top)
+        if not 1 <= top <= 128:
+            raise ValueError("top is %d, not 1 to 128" % top)
+        if labels is not None:
+            labels = numpy.asarray(labels, numpy.int32).reshape(-1)
+            if len(labels) != x.shape[0]:
+                raise ValueError("%d labels for %d samples" %
+                                 (len(labels), x.shape[0]))
+        if not x.shape[0]:
+            raise ValueError("no samples")
+        parts = []
+        with self._lock:
+            on_gpu = self._in.devmem is not None and self._in.on_gpu
+            run = self._top_device if on_gpu else self._top_numpy
+            for i in range(0, x.shape[0], self.batch_size):
+                some = None if labels is None else \
+                    labels[i:i + self.batch_size]
+                parts.append(run(x[i:i + self.batch_size], some, top))
+        ans = {k: numpy.concatenate([p[k] for p in parts])
+               for k in parts[0]}
+        if labels is None:
+            del ans["logprob"]
+        return ans
 
 
 # -- flat export for the standalone C++ engine (mzserve) --------------------
@@ -235,6 +352,14 @@ def export_flat(engine, outdir):
             rows = int(numpy.prod(f.input.shape)) // C
             lines.append("op lrn %d %d %r %r %r %d %d" %
                          (C, rows, f.alpha, f.beta, f.k, f.n, out_numel))
+        elif isinstance(f, normalization.LayerNormForward):
+            C = f.input.shape[-1]
+            rows = int(numpy.prod(f.input.shape)) // C
+            wn = tensor("w%d" % i, host(f.weights), "f32")
+            bn = tensor("b%d" % i, host(f.bias), "f32") \
+                if f.include_bias else "-"
+            lines.append("op layernorm %s %s %d %d %r %d" %
+                         (wn, bn, C, rows, float(f.eps), out_numel))
         elif isinstance(f, act_mod.ActivationForward):
             lines.append("op act %d" % f.ACTIVATION)
         else:
@@ -255,6 +380,13 @@ def export_flat(engine, outdir):
 def serve(engine, port=8080):
     from http.server import BaseHTTPRequestHandler, HTTPServer
 
+    def finite(v):
+        """JSON has no infinities: they become null."""
+        if v.dtype.kind != "f":
+            return v.tolist()
+        return numpy.where(numpy.isfinite(v), v.astype(object),
+                           None).tolist()
+
     class Handler(BaseHTTPRequestHandler):
         def do_POST(self):
             try:
@@ -265,6 +397,9 @@ def serve(engine, port=8080):
                 if want_labels:
                     resp = {"labels":
                             engine.predict_labels(x).tolist()}
+                elif "top" in req:
+                    resp = {k: finite(v) for k, v in engine.predict_top(
+                        x, req["top"], req.get("labels")).items()}
                 else:
                     resp = {"outputs": engine.predict(x).tolist()}
                 body = json.dumps(resp).encode()

@@ -7,9 +7,9 @@ set -e
 cd "$(dirname "$0")"
 SRCS="mzserve.cpp ../ops/hip/gemm.hip ../ops/hip/gemm8.hip \
       ../ops/hip/elementwise.hip ../ops/hip/softmax.hip \
-      ../ops/hip/pool_lrn.hip"
+      ../ops/hip/pool_lrn.hip ../ops/hip/layer_norm.hip"
 DEPS="$SRCS ../ops/hip/api.h ../ops/hip/common.h ../ops/hip/loaders.h \
-      ../ops/hip/sgd_multi.h build.sh"
+      ../ops/hip/sgd_multi.h ../ops/hip/rows.h build.sh"
 if [ -x mzserve ]; then
   stale=0
   for f in $DEPS; do

@@ -10,14 +10,14 @@
 //                  bf16, fp32 biases), 16-B aligned offsets
 // Links the SAME kernel translation units as the _mzk extension
 // (gemm.hip / gemm8.hip / pool_lrn.hip / elementwise.hip /
-// softmax.hip) — no torch, no Python: hip runtime only.  The whole
+// softmax.hip / layer_norm.hip) — no torch, no Python: hip runtime only.  The whole
 // forward pass is captured into one hipGraph after a warmup batch and
 // replayed per batch (launch-bound regime), mirroring the Python
 // InferenceEngine.
 //
 // Build (done by __graft_entry__.build() / serve/build.sh):
 //   hipcc -O3 -std=c++17 --offload-arch=gfx950 mzserve.cpp \
-//     ../ops/hip/{gemm,gemm8,elementwise,softmax,pool_lrn}.hip -o mzserve
+//     ../ops/hip/{gemm,gemm8,elementwise,softmax,pool_lrn,layer_norm}.hip -o mzserve
 //
 // Run:
 //   ./mzserve <export_dir> [--input in.f32.bin] [--out out.f32.bin]
@@ -55,6 +55,8 @@ void pool_fwd_launch(const unsigned short*, unsigned short*,
 void lrn_fwd_launch(const unsigned short*, unsigned short*, float*, long,
                     int, float, float, float, int, hipStream_t);
 void softmax_launch(float*, int*, int, int, hipStream_t);
+void layer_norm_fwd_launch(int, RowsIn, RowsOut, const float*, const float*,
+                           float*, float*, long, int, float, hipStream_t);
 void act_fwd_launch(unsigned short*, long, int, hipStream_t);
 
 #define HIP_OK(call)                                                     \
@@ -93,7 +95,8 @@ struct TensorRef {
 };
 
 struct Op {
-  std::string kind;          // fc | softmax | conv | pool | lrn | act
+  std::string kind;          // fc | softmax | conv | pool | lrn |
+                             // layernorm | act
   std::string w, bias;       // tensor names ("-" = none)
   int act = 0;
   int M = 0, N = 0, K = 0;   // fc
@@ -101,8 +104,9 @@ struct Op {
   int rows = 0, cols = 0;    // softmax
   std::vector<int> desc;     // conv (13) / pool (11)
   int mode = 0;              // pool
-  int C = 0;                 // lrn
+  int C = 0;                 // lrn, layernorm
   long lrn_rows = 0;
+  float eps = 0;             // layernorm
   float alpha = 0, beta = 0, k = 0;
   int win = 0;
   long out_numel = 0;
@@ -168,6 +172,14 @@ Model parse_manifest(const std::string& dir) {
       } else if (op.kind == "lrn") {
         ss >> op.C >> op.lrn_rows >> op.alpha >> op.beta >> op.k >>
             op.win >> op.out_numel;
+      } else if (op.kind == "layernorm") {
+        ss >> op.w >> op.bias >> op.C >> op.lrn_rows >> op.eps >>
+            op.out_numel;
+        if (!ss || op.C < 1 || op.lrn_rows < 0 ||
+            op.out_numel != op.lrn_rows * op.C) {
+          std::fprintf(stderr, "mzserve: bad layernorm op\n");
+          std::exit(1);
+        }
       } else if (op.kind == "act") {
         ss >> op.act;
       } else {
@@ -232,6 +244,19 @@ struct Engine {
                      "weights.bin (%zu B)\n", kv.first.c_str(), bytes,
                      t.offset, blob.size());
         std::exit(1);
+      }
+    }
+    for (const Op& op : m.ops) {
+      if (op.kind != "layernorm") continue;
+      for (const std::string& name : {op.w, op.bias}) {
+        if (name == "-") continue;
+        auto it = m.tensors.find(name);
+        if (it == m.tensors.end() || it->second.dtype != "f32" ||
+            it->second.numel != op.C) {
+          std::fprintf(stderr, "mzserve: layernorm of %d columns: bad "
+                               "tensor %s\n", op.C, name.c_str());
+          std::exit(1);
+        }
       }
     }
     HIP_OK(hipStreamCreateWithFlags(&stream, hipStreamNonBlocking));
@@ -305,6 +330,21 @@ struct Engine {
         lrn_fwd_launch((const unsigned short*)cur,
                        (unsigned short*)outs[i], nullptr, op.lrn_rows,
                        op.C, op.alpha, op.beta, op.k, op.win, stream);
+        cur = outs[i];
+        cur_numel = op.out_numel;
+        cur_f32 = false;
+      } else if (op.kind == "layernorm") {
+        if (cur_f32 || cur_numel != op.out_numel) {
+          std::fprintf(stderr, "mzserve: layernorm of %ld bf16 values "
+                               "after %ld %s ones\n", op.out_numel,
+                       cur_numel, cur_f32 ? "f32" : "bf16");
+          std::exit(1);
+        }
+        layer_norm_fwd_launch(ROW_BF16, RowsIn{cur, op.C},
+                              RowsOut{outs[i], op.C},
+                              (const float*)tptr(op.w),
+                              (const float*)tptr(op.bias), nullptr, nullptr,
+                              op.lrn_rows, op.C, op.eps, stream);
         cur = outs[i];
         cur_numel = op.out_numel;
         cur_f32 = false;
