@@ -134,6 +134,51 @@ def test_partial_overlaps_are_refused():
             t(4, 2, dtype=f4), x.view(torch.bfloat16)[:, :8])
 
 
+def test_outputs_over_other_arrays_are_refused():
+    """No output may lie over another one, nor over what is read."""
+    x, y, w = t(4, 8), t(4, 8), t(8, dtype=f4)
+    m, r = t(4, dtype=f4), t(4, dtype=f4)
+    one = "mean and rstd overlap|rstd and mean overlap"
+    refused(one, ops.layer_norm_fwd, x, y, w, None, m, m)
+    refused("weights", ops.layer_norm_fwd, x, y, w, None, w[:4], r)
+    z = t(4, 8, dtype=f4)
+    refused("bias", ops.layer_norm_fwd, z, t(4, 8, dtype=f4), None, w, w[4:],
+            r)
+    refused("out and mean", ops.layer_norm_fwd, t(4, 8, dtype=f4), z, w,
+            None, z.view(-1)[8:12], r)
+    refused("grad_w and grad_b", ops.layer_norm_bwd, x, y, None, m, r, None,
+            w, w)
+    refused("weights", ops.layer_norm_bwd, x, y, w, m, r, None, w)
+    refused("mean", ops.layer_norm_bwd, z[:4, :4], t(4, 4, dtype=f4), None,
+            m, r, None, m)
+    e, i, p = t(4, dtype=f4), t(4, 2, dtype=i4), t(4, 2, dtype=f4)
+    lab = t(4, dtype=i4)
+    f = ops.token_logprobs
+    refused("logprob and entropy", f, x, lab, e, e)
+    refused("labels", f, x, lab, lab.view(f4))
+    refused("top_idx and top_logprob", f, x, top_idx=i,
+            top_logprob=i.view(f4))
+    refused("logits", f, z, entropy=z[1, :4])
+    d = ops.eval_distill
+    refused("top_logit", d, x, i, p, y, p.view(-1)[:4])
+    refused("labels", d, x, i, p, y, None, labels=lab, n_err=lab)
+    refused("top_idx", d, x, i, p, y, None, labels=lab, n_err=i)
+    refused("loss", d, z, i, p, z, z[3, 4:])
+    # beside each other, or between a matrix's rows
+    both = t(12, dtype=f4)
+    refused("not on a GPU", f, x, lab, both[:4], both[4:8])
+    wide = t(4, 16, dtype=f4)
+    refused("not on a GPU", f, wide[:, :8], entropy=wide[0, 8:12])
+    refused("overlap", f, wide[:, :8], entropy=wide[0, 7:11])
+    refused("overlap", f, wide[:, :8],
+            entropy=wide.view(-1)[14:18])
+
+
+def test_token_logprobs_class_limit():
+    refused("at most 2.24", ops.token_logprobs, t(1, (1 << 24) + 1),
+            entropy=t(1, dtype=f4))
+
+
 def test_token_logprobs_refusals():
     x = t(4, 50)
     f = ops.token_logprobs

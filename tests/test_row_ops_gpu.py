@@ -383,6 +383,23 @@ def test_token_logprobs_top(R, C, name, top):
     check_logprobs(tx, [C - 1] * R, run_logprobs(tx, [C - 1] * R, top))
 
 
+@pytest.mark.parametrize("R,C,name", [
+    (1, 600011, "bf16"),       # as many parts as there are, 128 of each
+    (1, 300007, "f32"),
+    (1, (1 << 24) - 3, "f16"),
+    (600, (1 << 20) - 5, "bf16"),   # the longest parts, many rows
+    (600, (1 << 19) - 3, "f32"),
+    (600, (1 << 20) + 1, "f16")])
+def test_token_logprobs_long_rows(R, C, name):
+    """(one row again and again: a stride of 0)"""
+    tx = rows_of(logits_case(1, C, 11), TYPES[name])
+    for top in (128, 3):
+        out = run_logprobs(tx.expand(R, C), [C - 1] * R, top)
+        check_logprobs(tx, [C - 1], [t[:1] for t in out])
+        for t in out:
+            assert torch.equal(t, t[:1].expand_as(t))
+
+
 @pytest.mark.parametrize("C", [1, 3, 64, 1000, 20000, 60000, 140007])
 @pytest.mark.parametrize("name", sorted(TYPES))
 def test_token_logprobs_orders(C, name):

@@ -306,7 +306,7 @@ def _rows(t):
 def token_logprobs(logits, labels=None, logprob=None, entropy=None,
                    top_idx=None, top_logprob=None, batch=None):
     """Answers of rows of logits [..., V] (bf16, fp16 or fp32; rows
-    contiguous, any stride apart), each output optional:
+    contiguous, any stride apart; V at most 2^24), each output optional:
 
     * ``logprob`` fp32[rows]: log probability of ``labels`` int32[rows].  A
       label below 0 is none (0 is written); one of V or more gives NaN.
@@ -318,7 +318,8 @@ def token_logprobs(logits, labels=None, logprob=None, entropy=None,
     A logit of minus infinity forbids its class; a row of them has entropy 0
     and log probabilities of minus infinity.  A row with NaN or plus infinity
     gives NaN, and -1 for its classes.  Rows from ``batch`` on are padding:
-    they are not read, and hold zeros (``top_idx`` -1)."""
+    they are not read, and hold zeros (``top_idx`` -1).  No output may lie
+    over another one or over what is read."""
     x = _rows(logits)
     require().token_logprobs(x, labels, logprob, entropy, top_idx,
                              top_logprob,
@@ -336,7 +337,7 @@ def eval_distill(logits, top_idx, top_logit, err_out, loss=None, batch=None,
         err_out = d loss / d logits = t (p - q)
 
     ``err_out`` has the logits' type and shape and may be ``logits`` itself;
-    that of fp32 logits may be bf16.
+    that of fp32 logits may be bf16.  Other outputs lie apart from all else.
     Places with a negative class or a logit of minus infinity are empty; a
     class that is named twice has both shares.  A row without a named class,
     or whose logits are all minus infinity, has no loss and no gradient; one
@@ -402,7 +403,7 @@ def layer_norm_fwd(x, out, weights, bias, mean, rstd, eps=1e-5):
 
     x, out: bf16, fp16 or fp32, rows contiguous, any stride apart; ``out``
     may be ``x``.  weights, bias: fp32[C] or None; mean, rstd: fp32[rows],
-    written for the backward pass, or None."""
+    written for the backward pass, or None, and apart from all else."""
     require().layer_norm_fwd(_rows(x), _rows(out), weights, bias, mean,
                              rstd, float(eps))
 
@@ -412,7 +413,7 @@ def layer_norm_bwd(err_out, x, weights, mean, rstd, err_in, grad_w=None,
     """Backward of :func:`layer_norm_fwd` with the ``mean`` and ``rstd`` it
     wrote.  err_in (or None) may be ``err_out`` or ``x``; grad_w, grad_b:
     fp32[C] or None, sums over all rows, always in the same order
-    (``accumulate``: added to what they hold)."""
+    (``accumulate``: added to what they hold), apart from all else."""
     require().layer_norm_bwd(_rows(err_out), _rows(x), weights, mean, rstd,
                              None if err_in is None else _rows(err_in),
                              grad_w, grad_b, bool(accumulate))

@@ -543,24 +543,51 @@ void check_gpu(const char* op, const torch::Tensor& x) {
   TORCH_CHECK(x.is_cuda(), op, ": the tensors are not on a GPU");
 }
 
-// An output may be an input itself, element for element, or lie between its
-// rows, but not over a part of it.
-void check_overlap(const char* op, const char* name, const torch::Tensor& out,
-                   const torch::Tensor& in) {
-  const int64_t R = out.size(0), C = out.size(1);
-  if (R == 0) return;
-  const int64_t so = R == 1 ? 0 : out.stride(0) * out.element_size();
-  const int64_t si = R == 1 ? 0 : in.stride(0) * in.element_size();
-  const int64_t wo = C * out.element_size(), wi = C * in.element_size();
-  const char* po = static_cast<const char*>(out.data_ptr());
-  const char* pi = static_cast<const char*>(in.data_ptr());
-  bool over = po < pi + (R - 1) * si + wi && pi < po + (R - 1) * so + wo;
-  if (over && so == si && wo == wi && po == pi) over = false;
-  if (over && so == si && so > 0) {
-    const int64_t d = ((pi - po) % so + so) % so;   // in's rows after out's
-    over = d < wo || so - d < wi;
-  }
-  TORCH_CHECK(!over, op, ": ", name, " overlaps an input in part");
+// Memory that a call reads or writes: rows of `width` bytes, `step` apart
+struct Span {
+  const char* name;
+  const char* p;
+  int64_t rows, step, width;
+  bool written, matrix;
+};
+
+Span span(const char* name, const torch::Tensor& t, bool written) {
+  const int64_t R = t.size(0), e = t.element_size();
+  return Span{name, static_cast<const char*>(t.data_ptr()), R,
+              R > 1 ? t.stride(0) * e : 0, t.size(1) * e, written, true};
+}
+
+template <typename V>
+Span span(const char* name, const V* p, int64_t n, bool written) {
+  return Span{name, reinterpret_cast<const char*>(p), p ? 1 : 0, 0,
+              n * (int64_t)sizeof(V), written, false};
+}
+
+bool overlap(const Span& a, const Span& b) {
+  if (!a.rows || !b.rows || !a.width || !b.width) return false;
+  if (a.p >= b.p + (b.rows - 1) * b.step + b.width ||
+      b.p >= a.p + (a.rows - 1) * a.step + a.width)
+    return false;
+  if (a.rows > 1 && b.rows == 1) return overlap(b, a);
+  // one may lie between the rows of the other
+  if (b.step <= 0 || (a.rows > 1 && a.step != b.step)) return true;
+  if (a.rows == 1 && a.p < b.p) return true;
+  const int64_t d = ((a.p - b.p) % b.step + b.step) % b.step;
+  return d < b.width || d + a.width > b.step;
+}
+
+// An output may be an input matrix itself, element for element, or lie
+// between its rows; apart from that no output is over anything else.
+void check_apart(const char* op, std::initializer_list<Span> all) {
+  for (const Span* a = all.begin(); a != all.end(); ++a)
+    for (const Span* b = all.begin(); b != a; ++b) {
+      if (!(a->written || b->written) || !overlap(*a, *b)) continue;
+      const bool both = a->matrix && b->matrix;
+      if (both && a->p == b->p && a->step == b->step && a->width == b->width)
+        continue;
+      TORCH_CHECK(false, op, ": ", b->name, " and ", a->name, " overlap",
+                  both ? " in part" : "");
+    }
 }
 
 void layer_norm_fwd(torch::Tensor x, torch::Tensor y, Opt w, Opt b, Opt mean,
@@ -568,7 +595,6 @@ void layer_norm_fwd(torch::Tensor x, torch::Tensor y, Opt w, Opt b, Opt mean,
   const char* op = "layer_norm_fwd";
   check_rows(op, "x", x, x, x.scalar_type(), false);
   check_rows(op, "out", y, x, x.scalar_type(), true);
-  check_overlap(op, "out", y, x);
   TORCH_CHECK(eps >= 0 && eps < 1e30, op, ": eps is ", eps);
   const int type = row_type(op, x);
   const int64_t R = x.size(0), C = x.size(1);
@@ -576,6 +602,9 @@ void layer_norm_fwd(torch::Tensor x, torch::Tensor y, Opt w, Opt b, Opt mean,
   const float* bp = array<float>(op, "bias", b, C, x);
   float* mp = array<float>(op, "mean", mean, R, x);
   float* rp = array<float>(op, "rstd", rstd, R, x);
+  check_apart(op, {span("out", y, true), span("mean", mp, R, true),
+                   span("rstd", rp, R, true), span("x", x, false),
+                   span("weights", wp, C, false), span("bias", bp, C, false)});
   check_gpu(op, x);
   c10::DeviceGuard guard(x.device());
   layer_norm_fwd_launch(type, rows_in(x), rows_out(y), wp, bp, mp, rp, R,
@@ -591,8 +620,6 @@ void layer_norm_bwd(torch::Tensor dy, torch::Tensor x, Opt w,
   RowsOut out{nullptr, 0};
   if (dx.has_value()) {
     check_rows(op, "err_input", *dx, x, x.scalar_type(), true);
-    check_overlap(op, "err_input", *dx, x);
-    check_overlap(op, "err_input", *dx, dy);
     out = rows_out(*dx);
   }
   const int type = row_type(op, x);
@@ -602,6 +629,12 @@ void layer_norm_bwd(torch::Tensor dy, torch::Tensor x, Opt w,
   const float* rp = array<float>(op, "rstd", rstd, R, x);
   float* dwp = array<float>(op, "grad_w", dw, C, x);
   float* dbp = array<float>(op, "grad_b", db, C, x);
+  check_apart(op, {dx.has_value() ? span("err_input", *dx, true)
+                                  : span("err_input", mp, 0, true),
+                   span("grad_w", dwp, C, true), span("grad_b", dbp, C, true),
+                   span("err_output", dy, false), span("x", x, false),
+                   span("weights", wp, C, false), span("mean", mp, R, false),
+                   span("rstd", rp, R, false)});
   check_gpu(op, x);
   c10::DeviceGuard guard(x.device());
   torch::Tensor part;
@@ -649,6 +682,10 @@ void token_logprobs(torch::Tensor x, Opt labels, Opt logprob, Opt entropy,
   float* ep = array<float>(op, "entropy", entropy, R, x);
   int* ip = array<int>(op, "top_idx", top_idx, R * top, x);
   float* tp = array<float>(op, "top_logprob", top_lp, R * top, x);
+  check_apart(op, {span("logprob", gp, R, true), span("entropy", ep, R, true),
+                   span("top_idx", ip, R * top, true),
+                   span("top_logprob", tp, R * top, true),
+                   span("logits", x, false), span("labels", lp, R, false)});
   check_gpu(op, x);
   c10::DeviceGuard guard(x.device());
   torch::Tensor scratch;
@@ -673,7 +710,6 @@ void eval_distill(torch::Tensor x, torch::Tensor idx, torch::Tensor z,
                       err.scalar_type() == torch::kBFloat16;
   check_rows(op, "err_output", err, x,
              narrow ? torch::kBFloat16 : x.scalar_type(), true);
-  check_overlap(op, "err_output", err, x);
   const int64_t R = x.size(0), C = x.size(1);
   const int64_t live = live_rows(op, batch, R);
   TORCH_CHECK(tau >= 1e-3 && tau <= 1e3, op, ": temperature is ", tau,
@@ -695,6 +731,11 @@ void eval_distill(torch::Tensor x, torch::Tensor idx, torch::Tensor z,
   const int* lp = array<int>(op, "labels", labels, R, x);
   int* np = array<int>(op, "n_err", n_err,
                        n_err.has_value() ? n_err->numel() : 0, x);
+  check_apart(op, {span("err_output", err, true), span("loss", sp, R, true),
+                   span("n_err", np, 1, true), span("logits", x, false),
+                   span("top_idx", ip, R * top, false),
+                   span("top_logit", zp, R * top, false),
+                   span("labels", lp, R, false)});
   check_gpu(op, x);
   c10::DeviceGuard guard(x.device());
   torch::Tensor scratch;
