@@ -233,6 +233,29 @@ def test_predict_top_matches_predict(tmp_path):
         eng.predict_top(x[:0], 3)
 
 
+def test_predict_top_labels_of_any_type(tmp_path):
+    """Whole numbers beyond 32 bits do not come round to a class; others are
+    refused."""
+    from veles.serving import InferenceEngine
+    eng = InferenceEngine(teacher_file(tmp_path), device=NumpyDevice())
+    x = numpy.random.RandomState(2).normal(0, 1, (3, 24))
+    want = eng.predict_top(x, 2, [3, 0, 9])["logprob"]
+    for dtype in (numpy.int8, numpy.uint8, numpy.int64, numpy.uint64):
+        got = eng.predict_top(x, 2, numpy.array([3, 0, 9], dtype))
+        numpy.testing.assert_array_equal(got["logprob"], want)
+    got = eng.predict_top(x, 2, numpy.array([1 << 32, -(1 << 32), 10]))
+    assert numpy.isnan(got["logprob"][[0, 2]]).all()
+    assert got["logprob"][1] == 0
+    got = eng.predict_top(x, 2, numpy.array([1 << 63, 3, 0], numpy.uint64))
+    assert numpy.isnan(got["logprob"][0])
+    for bad in ([1.5, 0, 0], [True, False, True], ["1", "2", "3"]):
+        with pytest.raises(ValueError, match="whole numbers"):
+            eng.predict_top(x, 2, bad)
+    for bad in (2.5, "3", None):
+        with pytest.raises(ValueError, match="top is"):
+            eng.predict_top(x, bad)
+
+
 def test_top_answers_over_http(tmp_path):
     import socket
     from veles import serving

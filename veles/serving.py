@@ -19,6 +19,7 @@ launch-bound, exactly the regime graph replay removes.
 """
 
 import json
+import numbers
 import threading
 
 import numpy
@@ -218,23 +219,31 @@ class InferenceEngine(object):
     def predict_top(self, x, top=5, labels=None):
         """The likeliest classes of each sample with their log probabilities:
         {"top": int32[n, top], "top_logprob": fp32[n, top], "entropy":
-        fp32[n]} and, for given ``labels``, "logprob": fp32[n].  ``top`` is 1
-        to 128; places beyond the number of classes hold -1 and minus
-        infinity."""
+        fp32[n]} and, for given ``labels``, "logprob": fp32[n] (0 for a
+        label below 0, NaN for one beyond the classes).  ``top`` is 1 to 128;
+        places beyond the number of classes hold -1 and minus infinity."""
         x = numpy.asarray(x, numpy.float32)
         if x.shape[1:] != tuple(self._in.shape[1:]):
             raise ValueError("sample shape %s != model input %s" %
                              (x.shape[1:], tuple(self._in.shape[1:])))
+        if not isinstance(top, numbers.Integral) or not 1 <= top <= 128:
+            raise ValueError("top is %r, not 1 to 128" % (top,))
         top = int(top)
-        if not 1 <= top <= 128:
-            raise ValueError("top is %d, not 1 to 128" % top)
+        if not x.shape[0]:
+            raise ValueError("no samples")
         if labels is not None:
-            labels = numpy.asarray(labels, numpy.int32).reshape(-1)
+            labels = numpy.asarray(labels).reshape(-1)
             if len(labels) != x.shape[0]:
                 raise ValueError("%d labels for %d samples" %
                                  (len(labels), x.shape[0]))
-        if not x.shape[0]:
-            raise ValueError("no samples")
+            if labels.dtype.kind not in "iu":
+                raise ValueError("labels are %s, not whole numbers" %
+                                 labels.dtype)
+            # (int32, of any type; beyond it there is no class either way)
+            beyond = labels > (1 << 31) - 1
+            labels = numpy.where(beyond, 0, labels).astype(numpy.int64)
+            labels[beyond] = (1 << 31) - 1
+            labels = numpy.maximum(labels, -1).astype(numpy.int32)
         parts = []
         with self._lock:
             on_gpu = self._in.devmem is not None and self._in.on_gpu
