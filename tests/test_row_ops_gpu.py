@@ -611,6 +611,45 @@ def test_eval_distill_special_rows(C, name):
         assert loss[7] == INF
 
 
+@pytest.mark.parametrize("C", [5001, 20001, 40000, 50001, 140007])
+@pytest.mark.parametrize("name", sorted(TYPES))
+@pytest.mark.parametrize("pad,shift", [(0, 0), (1, 3)])
+def test_eval_distill_many_long_rows(C, name, pad, shift):
+    """Rows enough not to be cut into parts, special ones among them, in
+    turn."""
+    R, turns, tau = 12, 7, 1.5
+    x = logits_case(R, C, 13)
+    idx, z = teacher_case(R, C, 100, 13)
+    x[0] = -INF
+    idx[1] = -1
+    idx[2] = C - 1 - numpy.arange(100) % 3      # the last ones, again
+    idx[3] = numpy.arange(100)                  # beside each other
+    x[4, C // 2] = numpy.nan
+    x[5] = -2.0 ** 15                           # far below 0, as one
+    x[6] += 3e4                                 # far above
+    x[7, :C // 2] = -INF
+    idx[7] = C // 2 + numpy.arange(100)
+    z[8, ::2] = -INF
+    x[9, C - 1] = 40.0                          # at the row's end alone
+    dtype = TYPES[name]
+    tx = rows_of(numpy.tile(x, (turns, 1)), dtype, pad, shift)
+    err = rows_of(numpy.full(tx.shape, 55.0), dtype, pad, shift)
+    loss = torch.full((R * turns,), 55.0, device="cuda")
+    labels = f64(tx).argmax(1)
+    labels[1::2] = (labels[1::2] + 1) % C
+    n = torch.zeros(1, dtype=torch.int32, device="cuda")
+    live = R * turns - 2
+    idx, z = numpy.tile(idx, (turns, 1)), numpy.tile(z, (turns, 1))
+    ops.eval_distill(tx, cuda(idx), cuda(z), err, loss, live, tau,
+                     torch.as_tensor(labels, dtype=torch.int32).cuda(), n)
+    # (rows of an odd length start at other places within 16 bytes each time,
+    # which is another order of their sums: equal to the bit they need not be)
+    check_distill(tx, f64(tx), idx, z, tau, err, loss, live)
+    rows = numpy.arange(live) % R
+    wrong = (numpy.arange(live) % 2 == 1) | (rows == 0) | (rows == 4)
+    assert n.item() == wrong.sum()
+
+
 @pytest.mark.parametrize("batch", [0, 1, 5, 6])
 @pytest.mark.parametrize("C", [100, 50001])
 def test_eval_distill_padded_batch(batch, C):

@@ -1209,6 +1209,11 @@ static dim3 parts_grid(int split, long rows) {
 #define LP_LEAST 4
 #define LP_BLOCKS 512
 
+// Packs of a thread at most that are held (4096 rows of 8000 fp32: 26.9 us,
+// streamed 30.8; 8192 of 8000 bf16 37.9, 42.0).  With 16 of them too few waves
+// fit a compute unit: 4096 x 20000 bf16 42.5 us, streamed 38.4.
+#define LP_HELD 8
+
 // How a call is laid out: parts of a row, elements of a part, and packs of
 // a thread where they are held (0: they stream past)
 struct LogprobsPlan {
@@ -1217,7 +1222,7 @@ struct LogprobsPlan {
 
 static LogprobsPlan logprobs_plan(int type, long rows, int cols) {
   const int n = type == ROW_F32 ? 4 : 8;
-  const long held = LP_THREADS * 16 * n;
+  const long held = LP_THREADS * LP_HELD * n;
   const long most = (long)LP_GROUPS * GROUP * n;
   long split = (cols + most - 1) / most;
   const long least = LP_THREADS * LP_LEAST * n;
@@ -1269,7 +1274,7 @@ static void logprobs_run(RowsIn x, LogprobsOut o, LogprobsPlan l, long rows,
       s, x, p, some, live, cols, l.size)
   if (some) {
     switch (l.nv) {
-      HELD(1) HELD(2) HELD(4) HELD(8) HELD(16)
+      HELD(1) HELD(2) HELD(4) HELD(8)
       default:
         if (o.top)
           STREAM(true);
@@ -1300,8 +1305,19 @@ void token_logprobs_launch(int type, RowsIn x, const int* labels,
 #undef RUN
 }
 
+// Rows are cut into parts up to as many rows: a part's sums are a pass of
+// their own, and what that costs is gained back where few compute units would
+// have work.  Whole rows of 131072 bf16 against parts: 1 row 17.0 and 9.8 us,
+// 30 rows 19.0 and 13.0, 60 22.1 and 19.6, 100 22.9 and 23.7, 200 26.3 and
+// 39.8.
+#define DISTILL_CUT 64
+
 // How a call is laid out: parts of a row, elements of a part, threads and
-// packs of a thread
+// packs of a thread.  Rows that 256 threads hold in 16 packs each are left to
+// them (4096 x 32000 bf16: 103 us; to 512 threads 107), since a workgroup's
+// loads, sums and stores then overlap another's; of longer ones as many
+// threads as hold them (2048 x 60000: 512 threads 101 us, 1024 124); what 1024
+// do not hold is read twice.
 struct DistillPlan {
   int split, size, threads, nv;
 };
@@ -1311,7 +1327,7 @@ static DistillPlan distill_plan(int type, long rows, int cols) {
   DistillPlan p{1, cols, 256, 1};
   const long least = 256 * 4 * n;
   long split = 1;
-  if (rows < 256)
+  if (rows <= DISTILL_CUT)
     while (split < 64 && rows * split < 512 && cols / (split + 1) >= least)
       ++split;
   if (split > 1) {
