@@ -166,6 +166,33 @@ def test_layer_norm(R, C, name, pad, shift):
         assert torch.isnan(buf[keep]).all()
 
 
+@pytest.mark.parametrize("pad,shift", [(0, 0), (1, 3)])
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("R,C", [
+    (300001, 5), (200003, 24), (70001, 96), (20003, 300), (9001, 1000),
+    (4099, 2048), (2500, 4097), (1501, 8000), (600, 16384), (601, 17000),
+    (300, 33000)])
+def test_layer_norm_many_rows(R, C, name, pad, shift):
+    """Rows enough for several steps of every team, also over the inputs."""
+    dtype = TYPES[name]
+    x, dy, w, b = norm_case(R, C, dtype, 1)
+    tx, tdy = (rows_of(v, dtype, pad, shift) for v in (x, dy))
+    y, dx = torch.empty_like(tx), torch.empty_like(tx)
+    mean = torch.empty(R, device="cuda")
+    rstd = torch.empty(R, device="cuda")
+    ops.layer_norm_fwd(tx, y, cuda(w), cuda(b), mean, rstd, 1e-5)
+    check_norm_fwd(tx, w, b, y, mean, rstd, 1e-5, dtype)
+    dw, db = torch.empty(C, device="cuda"), torch.empty(C, device="cuda")
+    ops.layer_norm_bwd(tdy, tx, cuda(w), mean, rstd, dx, dw, db)
+    check_norm_bwd(tdy, tx, w, mean, rstd, dx, dw, db, dtype)
+    dw2, db2 = torch.empty_like(dw), torch.empty_like(db)
+    ops.layer_norm_bwd(tdy, tx, cuda(w), mean, rstd, tdy, dw2, db2)
+    assert torch.equal(tdy, dx)
+    assert torch.equal(dw, dw2) and torch.equal(db, db2)
+    ops.layer_norm_fwd(tx, tx, cuda(w), cuda(b), None, None, 1e-5)
+    assert torch.equal(tx, y)
+
+
 @pytest.mark.parametrize("R,C", [(3, 40), (600, 96), (5, 4096), (2, 20001)])
 @pytest.mark.parametrize("what", ["no_w", "no_b", "no_dx", "no_dw", "no_db",
                                   "only_dx", "no_stats"])
