@@ -10,35 +10,96 @@
 #include "rows.h"
 
 #define LN_THREADS 256
-// partial column sums of long rows that a backward pass leaves to be joined
-#define LN_PARTS 256
+#define LN_LONG 1024
+// Partial column sums of long rows that a backward pass leaves to be joined:
+// one for each 32 rows within these bounds (1024 x 40000 bf16 with 32 of them
+// 110 us, 64 117, 128 127, 256 154, since each is as long as two rows of fp32;
+// 4096 x 17000 with 64 of them 183, 128 192; 16 x 40000 with 8 17, 16 21)
+#define LN_PARTS_FEW 8
+#define LN_PARTS 64
 
-// one workgroup to a row; the row is read three times, from the caches
-// after the first
+// A row that is too long for registers: f(first element, number) for each of
+// this thread's packs and for one of the elements behind the last pack.
+template <int N>
+struct Count {
+  static constexpr int n = N;
+};
+template <int N, typename F>
+__device__ __forceinline__ void over_row(int cols, F f) {
+  const int packs = cols / N, single = packs * N + threadIdx.x;
+#pragma unroll 2
+  for (int p = threadIdx.x; p < packs; p += LN_LONG) f(p * N, Count<N>());
+  if (single < cols) f(single, Count<1>());
+}
+template <typename T, int N>
+__device__ __forceinline__ void get_some(float* e, const T* x, Count<N>) {
+  if constexpr (N == 1) {
+    e[0] = (float)x[0];
+  } else {
+    Pack<T> v;
+    v.load(x);
+    v.get(e);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void put_some(T* y, const float* e, Count<N>) {
+  if constexpr (N == 1) {
+    y[0] = from_f<T>(e[0]);
+  } else {
+    Pack<T> v;
+    v.set(e);
+    v.store(y);
+  }
+}
+
+// (16 bytes at a time, which a loop over p[k] does not become)
+template <int N>
+__device__ __forceinline__ void get_param(float* v, const float* p, int j,
+                                          float none, Count<N>) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = none;
+  if (p) __builtin_memcpy(v, p + j, sizeof(float) * N);
+}
+
+// One workgroup to such a row; it is read three times (backward: twice), from
+// the caches after the first, 16 bytes at a time.  1024 x 40000 bf16: 54 us,
+// 3.0 TB/s of one read and one write (with single elements, or the parameters
+// one by one, 175 to 260); bound by the waits between its three readings.
 template <typename T>
-__global__ __launch_bounds__(LN_THREADS) void ln_fwd_k(
+__global__ __launch_bounds__(LN_LONG) void ln_fwd_k(
     RowsIn x_, RowsOut y_, const float* __restrict__ w,
     const float* __restrict__ b, float* __restrict__ mean,
     float* __restrict__ rstd, long rows, int cols, float eps) {
-  __shared__ float tmp[LN_THREADS / WAVE];
+  __shared__ float tmp[LN_LONG / WAVE];
+  constexpr int N = Pack<T>::N;
   for (long row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* x = (const T*)x_.p + row * x_.stride;
     T* y = (T*)y_.p + row * y_.stride;
-    float s = 0.f;
-    for (int j = threadIdx.x; j < cols; j += LN_THREADS) s += (float)x[j];
+    float s = 0.f, v = 0.f;
+    over_row<N>(cols, [&](int j, auto count) {
+      float e[count.n];
+      get_some(e, x + j, count);
+#pragma unroll
+      for (int k = 0; k < count.n; ++k) s += e[k];
+    });
     const float mu = block_sum(s, tmp) / cols;
-    float v = 0.f;
-    for (int j = threadIdx.x; j < cols; j += LN_THREADS) {
-      const float d = (float)x[j] - mu;
-      v += d * d;
-    }
+    over_row<N>(cols, [&](int j, auto count) {
+      float e[count.n];
+      get_some(e, x + j, count);
+#pragma unroll
+      for (int k = 0; k < count.n; ++k) v = fmaf(e[k] - mu, e[k] - mu, v);
+    });
     const float r = 1.f / sqrtf(block_sum(v, tmp) / cols + eps);
-    for (int j = threadIdx.x; j < cols; j += LN_THREADS) {
-      float h = ((float)x[j] - mu) * r;
-      if (w) h *= w[j];
-      if (b) h += b[j];
-      y[j] = from_f<T>(h);
-    }
+    over_row<N>(cols, [&](int j, auto count) {
+      float e[count.n], gain[count.n], shift[count.n];
+      get_some(e, x + j, count);
+      get_param(gain, w, j, 1.f, count);
+      get_param(shift, b, j, 0.f, count);
+#pragma unroll
+      for (int k = 0; k < count.n; ++k)
+        e[k] = fmaf((e[k] - mu) * r, gain[k], shift[k]);
+      put_some(y + j, e, count);
+    });
     if (threadIdx.x == 0) {
       if (mean) mean[row] = mu;
       if (rstd) rstd[row] = r;
@@ -47,35 +108,51 @@ __global__ __launch_bounds__(LN_THREADS) void ln_fwd_k(
 }
 
 template <typename T>
-__global__ __launch_bounds__(LN_THREADS) void ln_bwd_k(
+__global__ __launch_bounds__(LN_LONG) void ln_bwd_k(
     RowsIn dy_, RowsIn x_, const float* __restrict__ w,
     const float* __restrict__ mean, const float* __restrict__ rstd,
     RowsOut dx_, long rows, int cols) {
-  __shared__ float tmp[LN_THREADS / WAVE];
+  __shared__ float tmp[LN_LONG / WAVE];
+  constexpr int N = Pack<T>::N;
   for (long row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* dy = (const T*)dy_.p + row * dy_.stride;
     const T* x = (const T*)x_.p + row * x_.stride;
     T* dx = (T*)dx_.p + row * dx_.stride;
     const float mu = mean[row], r = rstd[row];
     float s1 = 0.f, s2 = 0.f;
-    for (int j = threadIdx.x; j < cols; j += LN_THREADS) {
-      const float g = (float)dy[j] * (w ? w[j] : 1.f);
-      s1 += g;
-      s2 += g * (((float)x[j] - mu) * r);
-    }
+    over_row<N>(cols, [&](int j, auto count) {
+      float e[count.n], g[count.n], gain[count.n];
+      get_some(e, x + j, count);
+      get_some(g, dy + j, count);
+      get_param(gain, w, j, 1.f, count);
+#pragma unroll
+      for (int k = 0; k < count.n; ++k) {
+        const float d = g[k] * gain[k];
+        s1 += d;
+        s2 = fmaf(d, (e[k] - mu) * r, s2);
+      }
+    });
     s1 = block_sum(s1, tmp) / cols;
     s2 = block_sum(s2, tmp) / cols;
-    for (int j = threadIdx.x; j < cols; j += LN_THREADS) {
-      const float g = (float)dy[j] * (w ? w[j] : 1.f);
-      const float h = ((float)x[j] - mu) * r;
-      dx[j] = from_f<T>(r * (g - s1 - h * s2));
-    }
+    over_row<N>(cols, [&](int j, auto count) {
+      float e[count.n], g[count.n], gain[count.n];
+      get_some(e, x + j, count);
+      get_some(g, dy + j, count);
+      get_param(gain, w, j, 1.f, count);
+#pragma unroll
+      for (int k = 0; k < count.n; ++k) {
+        const float d = g[k] * gain[k];
+        g[k] = r * (d - s1 - (e[k] - mu) * r * s2);
+      }
+      put_some(dx + j, g, count);
+    });
   }
 }
 
-// column sums of dy xh and dy over this workgroup's rows: one thread to a
+// Column sums of dy xh and dy over this workgroup's rows: one thread to a
 // pack of columns (the last one ends with the row), part[blockIdx.y] =
-// [2][cols]
+// [2][cols].  With ln_bwd_k and ln_join_k, 1024 x 40000 bf16: 110 us, 2.2 TB/s
+// of dy, x and dx once; they are read twice.
 template <typename T>
 __global__ __launch_bounds__(LN_THREADS) void ln_cols_k(
     RowsIn dy_, RowsIn x_, const float* __restrict__ mean,
@@ -115,7 +192,8 @@ __global__ __launch_bounds__(LN_THREADS) void ln_cols_k(
 }
 
 // The partial sums [parts][2][cols] joined, always in the same order: 32 of
-// the 2 cols columns to a workgroup, 8 slices of the parts
+// the 2 cols columns to a workgroup, 8 slices of the parts (256 parts of 4096
+// columns, 8 MB: 4.8 us, of which 4 are the launch and one load's delay)
 #define LN_SLICES 8
 __global__ __launch_bounds__(LN_THREADS) void ln_join_k(
     const float* __restrict__ part, int parts, float* __restrict__ dw,
@@ -298,7 +376,8 @@ __device__ __forceinline__ void wait_loads() {
 
 // In each step the next one's loads come before this one's stores: memory
 // operations are waited for in their order, and what waits for a load would
-// otherwise wait for stores to reach memory.  For the same reason nothing
+// otherwise wait for stores to reach memory (16384 x 4096 bf16: 61 us before,
+// 51 so, 5.2 TB/s, where a bare copy reaches 6.5).  For the same reason nothing
 // after those loads is on a condition; the last step is apart.
 template <typename T, int THREADS, int TEAM, int NV, bool EXACT, bool TINY>
 __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
@@ -378,7 +457,9 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
 }
 
 // The backward pass of the same teams; part[block] = [2][cols], the
-// workgroup's column sums.  SUMS: dw or db is asked for, DX: dx is.
+// workgroup's column sums.  SUMS: dw or db is asked for, DX: dx is.  16384 x
+// 4096 bf16 with the joining: 82 us, 4.9 TB/s; bound by memory and by the one
+// workgroup that a compute unit has.
 template <typename T, int THREADS, int TEAM, int NV, bool EXACT, bool SUMS,
           bool DX, bool TINY>
 __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
@@ -386,7 +467,6 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
     const float* __restrict__ mean, const float* __restrict__ rstd,
     RowsOut dx_, float* __restrict__ part, long rows, int cols) {
   constexpr int N = Pack<T>::N, E = NV * N;
-  constexpr bool AHEAD = NV < 8;
   __shared__ float tmp[4 * (THREADS / WAVE)];
   TeamSum<THREADS, TEAM, 2> sum{tmp, 0};
   const Slots<T, TEAM, NV, TINY> at(cols);
@@ -456,12 +536,11 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
       }
       out[i].set(g);
     }
-    if (AHEAD && !last) load(row + steps.teams);
+    if (!last) load(row + steps.teams);
     if (last && row >= rows) return;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       at.store(out[i], (T*)dx_.p + row * dx_.stride, i);
-    if (!AHEAD && !last) load(row + steps.teams);
   };
   load(steps.start + steps.mine);
   at.load_param(gain, w, 1.f);
@@ -507,13 +586,20 @@ static unsigned row_grid(long rows) {
   return (unsigned)(rows < 65536 ? rows : 65536);
 }
 
-// Rows of as many elements are held by teams: of 8 a lane up to 8192, then
-// of 16 and 32 (forward; backward 16, or 32 without the column sums).
+// Rows of up to LN_MOST elements are held by teams, forward, and up to
+// LN_MOST_SUMS backward: of 8 a lane as far as 1024 lanes go, then 16 and 32.
+// 2048 x 32000 bf16 forward: held 62 us, read three times 83.  Backward 4096 x
+// 16000: held 99, read twice 154; 32 elements a lane have no registers for the
+// sums, and without them were slower than reading twice (2048 x 32000: 219,
+// 179).  With 16 elements a lane from the start: 16384 x 4096 forward 56
+// instead of 51 us, 8000 x 1000 9.3 instead of 8.2 (65536 x 1000, where the
+// barriers of two waves weigh more, 54.6 instead of 59.9), backward 65536 x
+// 1000 87 instead of 78, 193600 x 96 31 instead of 27.
 #define LN_MOST 32768
 #define LN_MOST_SUMS 16384
 // Workgroups at most: 2048 of 256 threads forward (16384 x 4096 bf16 in 51
 // us, with 4096 of them 71, 8192 87).  Backward 256 of 1024 threads, one to a
-// compute unit, so that few column sums are left to be joined (84 us; 512 of
+// compute unit, so that few column sums are left to be joined (82 us; 512 of
 // them, in turns, 90; 128 118).
 #define LN_FORWARD 2048
 #define LN_BACKWARD 256
@@ -558,7 +644,7 @@ static void ln_fwd_run(RowsIn x, RowsOut y, const float* w, const float* b,
   constexpr int N = Pack<T>::N;
   if (cols > LN_MOST) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(ln_fwd_k<T>), dim3(row_grid(rows)),
-                       dim3(LN_THREADS), 0, s, x, y, w, b, mean, rstd, rows,
+                       dim3(LN_LONG), 0, s, x, y, w, b, mean, rstd, rows,
                        cols, eps);
     return;
   }
@@ -592,7 +678,11 @@ void layer_norm_fwd_launch(int type, RowsIn x, RowsOut y, const float* w,
 
 // workgroups of a backward pass, or partial sums that it leaves
 static long ln_parts(long rows, int cols) {
-  if (cols > LN_MOST_SUMS) return rows < LN_PARTS ? rows : LN_PARTS;
+  if (cols > LN_MOST_SUMS) {
+    long n = rows < LN_PARTS_FEW ? rows : LN_PARTS_FEW;
+    if (n < rows / 32) n = rows / 32;
+    return n < LN_PARTS ? n : LN_PARTS;
+  }
   long n = 0;
 #define GRID(THREADS, TEAM, E) n = team_grid(rows, 1024 / TEAM, LN_BACKWARD)
   LN_TEAMS(cols, GRID);
@@ -623,14 +713,11 @@ static void ln_bwd_run(RowsIn dy, RowsIn x, const float* w,
                          rows, cols);
       HIP_CHECK_LAST();
     }
-    if (!dx.p) return;
-    if (cols > LN_MOST) {
+    if (dx.p)
       hipLaunchKernelGGL(HIP_KERNEL_NAME(ln_bwd_k<T>), dim3(row_grid(rows)),
-                         dim3(LN_THREADS), 0, s, dy, x, w, mean, rstd, dx,
+                         dim3(LN_LONG), 0, s, dy, x, w, mean, rstd, dx,
                          rows, cols);
-      return;
-    }
-    sums = false;
+    return;
   }
   const dim3 grid((unsigned)ln_parts(rows, cols));
 #define RUN2(TEAM, E, EXACT, SUMS, DX, TINY)                                 \
@@ -640,7 +727,7 @@ static void ln_bwd_run(RowsIn dy, RowsIn x, const float* w,
       grid, dim3(1024), 0, s, dy, x, w, mean, rstd, dx, part, rows, cols)
 #define RUN(THREADS, TEAM, E)                                                \
   if constexpr (E == 32)                                                     \
-    RUN2(TEAM, E, false, false, true, false);                                \
+    return;                                                                  \
   else if (cols % N == 0 && sums && dx.p)                                    \
     RUN2(TEAM, E, true, true, true, false);                                  \
   else if (sums && dx.p)                                                     \
