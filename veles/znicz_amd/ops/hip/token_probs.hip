@@ -573,7 +573,12 @@ struct Place {
   }
 };
 
-// One workgroup to a part of a row, which it holds in registers
+// One workgroup to a part of a row, which it holds in registers, so that the
+// alternatives are found without reading it again.  8192 x 8000 bf16, 20 of
+// them: 38 us, 3.5 TB/s; 4096 x 8000 fp32 27 us, 4.8 TB/s.  Bound by the
+// delays of its steps one after another (load, sums, bound, order), which the
+// other workgroups of the compute unit cover as far as they fit; 256 x 1000
+// fp32 takes 4.5 us, of which 2.3 are a launch.
 template <typename T, int NV>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_held_k(
     RowsIn x_, PartOut p, long rows, long live, int cols, int size) {
@@ -651,6 +656,12 @@ __device__ __forceinline__ void max_of_eight_lanes(float* h) {
 // One workgroup to a part of a row that streams past it, four packs of a
 // thread at a time.  The largest value of each eight packs (128 bytes) stays
 // in LDS; for the alternatives those are read again that reach the bound.
+// 4096 x 50001 bf16, 20 alternatives: 77 us, 5.2 TB/s; 2048 x 131072, 64 of
+// them: 96 us, 5.6 TB/s, of 6.9 that bare loads reach.  Bound by memory, and
+// for some 10 us by the alternatives, which the workgroups of a compute unit
+// come to at about the same time.  Loads of the next four packs before the
+// sums of these took 4% off a call without alternatives and nothing off one
+// with them, for 20 registers more.
 #define GROUP 8
 template <typename T, bool TOP>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
@@ -752,7 +763,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_stream_k(
 
 // A row's parts joined.  Each part's list is in order, so that the first few
 // of all lists, one to a thread, have a bound as the threads' largest values
-// have within a part.
+// have within a part.  One row of 131072 bf16 in 16 parts, with the parts: 8.7
+// us in a graph, 5 alternatives; bound by two launches and the steps' delays.
 template <typename T>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_join_k(
     RowsIn x_, LogprobsOut o, const Part* __restrict__ parts,
@@ -1033,7 +1045,12 @@ __device__ __forceinline__ void put_gradients(O* to, const float* g,
 
 // One workgroup to a row, or (JOINED) to a part of a row whose sums
 // distill_part_k has left.  The teacher's side is done by the first wave
-// while the row is under way.
+// while the row is under way.  2048 x 131072 bf16: 219 us, 4.9 TB/s of one
+// read and one write; 4096 x 32000: 103 us, 5.1 TB/s; 1023 x 50001 fp32: 79
+// us, 5.1 TB/s.  Bound by memory and by the turns that a row takes: a compute
+// unit has registers for one row of 256 KB, so that nothing is loaded while it
+// is stored (a copy laid out the same takes 192 us of the 219).  Loading the
+// next row into the registers that the gradients leave was no faster.
 template <typename T, typename O, int THREADS, int NV, bool JOINED>
 __global__ __launch_bounds__(THREADS) void distill_k(DistillArgs a) {
   __shared__ DistillSpace<THREADS> sp;
@@ -1155,7 +1172,9 @@ __global__ __launch_bounds__(THREADS) void distill_k(DistillArgs a) {
   }
 }
 
-// sums of a part of a row, and the row's logits of the teacher's classes
+// Sums of a part of a row, and the row's logits of the teacher's classes.  One
+// row of 131072 bf16 in 16 parts, with their gradients: 9.8 us, two launches
+// and the delays of their steps.
 template <typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS) void distill_part_k(DistillArgs a) {
   __shared__ Sums tmp[THREADS / WAVE];
@@ -1202,12 +1221,16 @@ static dim3 parts_grid(int split, long rows) {
 // parts of a row that are joined at most, and groups that a part may have
 #define LP_PARTS 64
 #define LP_GROUPS 16384
-// Few rows are cut until there are two workgroups for each compute unit, but
-// into parts of 4 packs a thread at least.  One row of 131072 bf16: 11.0 us
-// with 4 packs, 11.0 with 2; 600 rows: 38 us with two workgroups, 41 with
-// four, 39 with eight (the parts' own ends and their joining weigh more).
+// Fewer rows than LP_ROWS are cut until there are four workgroups for each
+// compute unit, but into parts of 4 packs a thread at least.  In a graph, rows
+// of 131072 bf16, 64 alternatives, whole and cut: 60 rows 26.1 and 18.5 us, 100
+// rows 27.2 and 22.3, 200 28.5 and 29.4, 300 31.1 and 32.2, 511 33.1 and 44.2;
+// of 50001, 20 alternatives: 100 rows 14.0 and 14.0, 200 14.4 and 16.6.  One
+// row with 5 alternatives: parts of 4 packs 8.8 us, 8 10.2, 2 8.8 (30 rows, 64
+// alternatives: 15.9, 16.9, 17.1).
 #define LP_LEAST 4
-#define LP_BLOCKS 512
+#define LP_ROWS 192
+#define LP_BLOCKS 1024
 
 // Packs of a thread at most that are held (4096 rows of 8000 fp32: 26.9 us,
 // streamed 30.8; 8192 of 8000 bf16 37.9, 42.0).  With 16 of them too few waves
@@ -1226,7 +1249,7 @@ static LogprobsPlan logprobs_plan(int type, long rows, int cols) {
   const long most = (long)LP_GROUPS * GROUP * n;
   long split = (cols + most - 1) / most;
   const long least = LP_THREADS * LP_LEAST * n;
-  while (split < LP_PARTS && rows * split < LP_BLOCKS &&
+  while (rows < LP_ROWS && split < LP_PARTS && rows * split < LP_BLOCKS &&
          cols / (split + 1) >= least)
     ++split;
   // whole packs to a part
