@@ -473,6 +473,40 @@ def test_token_logprobs_masks(C, name):
     assert torch.isnan(out[0][13])             # no such class
 
 
+@pytest.mark.parametrize("C", [16390, 50001, 140007])
+@pytest.mark.parametrize("name", sorted(TYPES))
+@pytest.mark.parametrize("top", [7, 128])
+def test_token_logprobs_many_long_rows(C, name, top):
+    """Rows enough not to be cut into parts, masked, in the worst orders."""
+    dtype = TYPES[name]
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    n = numpy.arange(C)
+    x = logits_case(16, C, 4)
+    x[0] = -INF
+    x[1, 1:] = -INF
+    x[2, :C - 1] = -INF
+    x[3] = low
+    x[4, C // 2] = numpy.nan
+    x[5, C - 1] = INF
+    x[6, ::2] = -INF
+    x[7, C // 3] = high
+    x[8] = 0.0
+    x[9] = n % 7
+    x[10] = n / 100.0
+    x[11] = numpy.where(n % 2, 0.0, -0.0)
+    x[12] = numpy.where(n % 4096 < 64, n % 64 * 1.0, -3.0)
+    x[13] = numpy.where(n < 40, -n * 1.0, -INF)
+    x[14] = -n / 100.0
+    turns = 13
+    tx = rows_of(numpy.tile(x, (turns, 1)), dtype, 0, 1)
+    labels = numpy.arange(16 * turns) * 37 % C
+    live = 16 * turns - 3
+    out = run_logprobs(tx, labels, top, live)
+    # (the first rows, at every place within 16 bytes, and the last ones)
+    check_logprobs(tx[:48], labels[:48], [t[:48] for t in out])
+    check_logprobs(tx[-20:], labels[-20:], [t[-20:] for t in out], 17)
+
+
 def test_token_logprobs_huge_offset():
     """Shifted logits have the same answers, whatever the shift."""
     rng = numpy.random.RandomState(0)
