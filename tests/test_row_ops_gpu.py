@@ -762,6 +762,30 @@ def test_eval_distill_counts_errors(C, name):
     assert n.tolist() == [want, 0]
 
 
+def test_eval_distill_of_no_rows():
+    x = torch.empty(0, 50, dtype=torch.bfloat16, device="cuda")
+    n = torch.tensor([4], dtype=torch.int32, device="cuda")
+    ops.eval_distill(x, torch.empty(0, 3, dtype=torch.int32, device="cuda"),
+                     torch.empty(0, 3, device="cuda"), torch.empty_like(x),
+                     torch.empty(0, device="cuda"), labels=torch.empty(
+                         0, dtype=torch.int32, device="cuda"), n_err=n)
+    assert n.item() == 4
+
+
+def test_more_rows_than_a_grid_has_in_a_dimension():
+    R, C = 70001, 6
+    tx = rows_of(logits_case(R, C, 12), torch.float32)
+    labels = numpy.arange(R) % 7 - 1
+    check_logprobs(tx, labels, run_logprobs(tx, labels, 2, R - 9), R - 9)
+    idx, z = teacher_case(2, C, 3)
+    idx, z = idx[numpy.arange(R) % 2], z[numpy.arange(R) % 2]
+    err, loss = run_distill(tx, idx, z, 2.0, R - 9)
+    # (the first rows, those about each 32768, and the last ones)
+    for lo, hi in ((0, 20), (32758, 32778), (65526, 65546), (R - 20, R)):
+        check_distill(tx[lo:hi], f64(tx[lo:hi]), idx[lo:hi], z[lo:hi], 2.0,
+                      err[lo:hi], loss[lo:hi], min(hi, R - 9) - lo)
+
+
 def test_eval_distill_gradient_by_differences():
     R, C, tau = 2, 30, 1.7
     tx = rows_of(logits_case(R, C, 8), torch.float32)
