@@ -335,14 +335,22 @@ struct Slots {
       v.store(row + at(i));
     }
   }
-  // parameters of the lane's columns
+  // parameters of the lane's columns, 16 bytes at a time
   __device__ __forceinline__ void load_param(float* v, const float* p,
                                              float none) const {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int k = 0; k < NV * N; ++k) v[k] = none;
+    if (!p) return;
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        v[i * N + k] = p && (!TINY || k < cols) ? p[at(i) + k] : none;
+    for (int i = 0; i < NV; ++i) {
+      if (TINY) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (k < cols) v[k] = p[k];
+      } else {
+        __builtin_memcpy(v + i * N, p + at(i), sizeof(float) * N);
+      }
+    }
   }
 };
 
@@ -458,7 +466,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
 
 // The backward pass of the same teams; part[block] = [2][cols], the
 // workgroup's column sums.  SUMS: dw or db is asked for, DX: dx is.  16384 x
-// 4096 bf16 with the joining: 82 us, 4.9 TB/s; bound by memory and by the one
+// 4096 bf16 with the joining: 79 us, 5.1 TB/s; bound by memory and by the one
 // workgroup that a compute unit has.
 template <typename T, int THREADS, int TEAM, int NV, bool EXACT, bool SUMS,
           bool DX, bool TINY>
@@ -556,22 +564,28 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
   // have the same columns
   constexpr int LANES = TEAM < WAVE ? TEAM : WAVE;     // of a wave
   constexpr int SETS = TEAM < WAVE ? THREADS / WAVE : THREADS / TEAM;
-  __shared__ float all[SETS][E * TEAM];
+  __shared__ alignas(16) float all[SETS][E * TEAM];
   const int set = TEAM < WAVE ? threadIdx.x / WAVE : threadIdx.x / TEAM;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-      float d = half ? db[k] : dw[k];
+    for (int i = 0; i < NV; ++i) {
+      float d[N];
 #pragma unroll
-      for (int off = LANES; off < WAVE; off *= 2) d += __shfl_xor(d, off);
+      for (int k = 0; k < N; ++k) {
+        d[k] = half ? db[i * N + k] : dw[i * N + k];
+#pragma unroll
+        for (int off = LANES; off < WAVE; off *= 2)
+          d[k] += __shfl_xor(d[k], off);
+      }
       if (TEAM >= WAVE || (threadIdx.x & (WAVE - 1)) < TEAM)
-        all[set][k * TEAM + at.lane] = d;
+        __builtin_memcpy(&all[set][(i * TEAM + at.lane) * N], d, sizeof(d));
     }
     __syncthreads();
     float* out = part + (2l * blockIdx.x + half) * cols;
+    // (in the columns' order, so that a wave's stores lie together)
     for (int a = threadIdx.x; a < E * TEAM; a += THREADS) {
-      const int c = at.column(a % TEAM, a / TEAM / N, a / TEAM % N);
+      const int c = at.column(a / N % TEAM, a / N / TEAM, a % N);
       if (c < 0) continue;
       float d = all[0][a];
 #pragma unroll
@@ -599,7 +613,7 @@ static unsigned row_grid(long rows) {
 #define LN_MOST_SUMS 16384
 // Workgroups at most: 2048 of 256 threads forward (16384 x 4096 bf16 in 51
 // us, with 4096 of them 71, 8192 87).  Backward 256 of 1024 threads, one to a
-// compute unit, so that few column sums are left to be joined (82 us; 512 of
+// compute unit, so that few column sums are left to be joined (79 us; 512 of
 // them, in turns, 90; 128 118).
 #define LN_FORWARD 2048
 #define LN_BACKWARD 256
