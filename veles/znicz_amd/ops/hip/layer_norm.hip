@@ -346,7 +346,7 @@ struct Slots {
       if (TINY) {
 #pragma unroll
         for (int k = 0; k < N; ++k)
-          if (k < cols) v[k] = p[k];
+          if (k < cols) v[i * N + k] = p[k];
       } else {
         __builtin_memcpy(v + i * N, p + at(i), sizeof(float) * N);
       }
