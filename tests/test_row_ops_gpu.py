@@ -410,6 +410,27 @@ def test_token_logprobs_top(R, C, name, top):
     check_logprobs(tx, [C - 1] * R, run_logprobs(tx, [C - 1] * R, top))
 
 
+@pytest.mark.parametrize("C", [129, 200, 255, 256, 257, 270, 400, 511, 513,
+                               700, 1000, 1023, 1025, 1039, 1500])
+@pytest.mark.parametrize("name", sorted(TYPES))
+@pytest.mark.parametrize("pad,shift", [(0, 0), (1, 5)])
+def test_token_logprobs_short_rows_of_many_alternatives(C, name, pad, shift):
+    """Fewer packs than threads, and than alternatives."""
+    rng = numpy.random.RandomState(C)
+    x = rng.normal(0, 3, (9, C))
+    x[1] = numpy.round(x[1])                    # equal values
+    x[2, rng.rand(C) < 0.8] = -INF
+    x[3, 130:] = -INF
+    x[4] = 2.0
+    x[5, :C // 2] += 100.0                      # all in the same packs
+    x[6, ::9] += 100.0
+    x[7, :] = -numpy.arange(C)
+    tx = rows_of(x, TYPES[name], pad, shift)
+    labels = numpy.arange(9) * 11 % C
+    for top in (33, 66, 128):
+        check_logprobs(tx, labels, run_logprobs(tx, labels, top))
+
+
 @pytest.mark.parametrize("R,C,name", [
     (1, 600011, "bf16"),       # as many parts as there are, 128 of each
     (1, 300007, "f32"),

@@ -573,6 +573,34 @@ struct Place {
   }
 };
 
+// Rows so short that half the threads or more have no pack: in place of each
+// thread's largest value that of each half, quarter, ... of a pack, as many as
+// there are threads, of which the bound is less often too low.  4096 x 1000
+// bf16 with 128 alternatives, for which 125 threads have too few values: 92 us
+// without, 29 so; 4096 x 500 70 and 26.  Not where there are many threads to an
+// alternative, or few classes in all (4096 x 1000, 20 of them: 13.9 us without,
+// 14.3 so; 6 x 72: 5.4, 5.8).
+template <typename T, int S = 2>
+__device__ __forceinline__ bool put_pieces(
+    const Held<T, LP_THREADS, 1>& h, int packs, int* high) {
+  constexpr int N = Pack<T>::N, LANES = LP_THREADS / S;
+  if (packs > LANES) return false;
+  if constexpr (S < N)
+    if (packs <= LANES / 2) return put_pieces<T, 2 * S>(h, packs, high);
+  if (threadIdx.x < LANES) {
+    float e[N];
+    h.v[0].get(e);
+#pragma unroll
+    for (int g = 0; g < S; ++g) {
+      float m = g ? -INFINITY : h.rest;
+#pragma unroll
+      for (int j = 0; j < N / S; ++j) m = fmaxf(m, e[g * (N / S) + j]);
+      high[g * LANES + threadIdx.x] = order_of(m);
+    }
+  }
+  return true;
+}
+
 // One workgroup to a part of a row, which it holds in registers, so that the
 // alternatives are found without reading it again.  8192 x 8000 bf16, 20 of
 // them: 38 us, 3.5 TB/s; 4096 x 8000 fp32 27 us, 4.8 TB/s.  Bound by the
@@ -600,7 +628,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_held_k(
   h.load(x, cut);
   float high[NV];
   Sums a = held_sums<true>(h, cut.packs, LOG2E, high);
-  sp.high[tid] = order_of(a.m);
+  bool pieces = false;
+  if constexpr (NV == 1)
+    if (at.n > 128 && cut.packs < 4 * p.o.top)
+      pieces = put_pieces<T>(h, cut.packs, sp.high);
+  if (!pieces) sp.high[tid] = order_of(a.m);
   a = join_block<true, LP_THREADS>(a, LOG2E, tmp);
   if (is_far(a.m, LOG2E)) a = far_sums(x, at.n, a.m, LOG2E, (float*)tmp);
   Row r;
