@@ -280,6 +280,16 @@ __device__ __forceinline__ float inv_sqrt(float v) {
   return small ? r * 0x1p50f : r;
 }
 
+// sum / cols to the nearest: the product with the rounded reciprocal `per` and
+// the rest that it leaves, which is exact.  The product alone is off by a step
+// for 3.0 at 1000 columns, say, and what a row of equal values then keeps of
+// itself is multiplied by a deviation of up to 1 / sqrt(eps).  (A sum that is
+// no number or infinite has no rest.)
+__device__ __forceinline__ float mean_of(float sum, int cols, float per) {
+  const float q = sum * per, rest = fmaf(-q, (float)cols, sum);
+  return rest == rest ? fmaf(rest, per, q) : q;
+}
+
 // Where a lane's packs of a row lie.  The last pack of a row that is no
 // whole number of packs ends with the row, so that its first elements are
 // the pack's before, too; a lane beyond the last pack has that one again.
@@ -418,7 +428,7 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_team_k(
       mu += at.has(i) ? q : 0.f;
     }
     sum(&mu);
-    mu *= per;
+    mu = mean_of(mu, cols, per);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float e[N], q = 0.f;
@@ -528,7 +538,7 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_team_k(
       return;
     }
     sum(s);
-    const float s1 = s[0] * per, s2 = s[1] * per;
+    const float s1 = mean_of(s[0], cols, per), s2 = mean_of(s[1], cols, per);
     Pack<T> out[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
