@@ -1,0 +1,51 @@
+"""What the distillation units and the engine leave behind on the GPU: the
+likeliest class beside the logits, a captured step after a change of the
+temperature, graphs and copies of the served answers."""
+
+import numpy
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("no GPU", allow_module_level=True)
+
+from test_distillation import build, mlp, save, teacher_file  # noqa: E402
+from test_distillation_answers import student  # noqa: E402
+from veles.backends import ROCmDevice  # noqa: E402
+
+
+def steps(tmp_path, graph, n=14):
+    """n training steps, the temperature changed after the eighth."""
+    from bench import _NullCtx
+    from veles.znicz_amd.hipgraph import GraphStepper
+    from veles.znicz_amd.parallel import GradientReducer
+    dev = ROCmDevice(0)
+    wf = student(tmp_path, dev, n_train=120, n_valid=0)
+    wf.grad_reducer = GradientReducer(_NullCtx(), dev)
+    st = GraphStepper(wf, warmup=2 if graph else 100)
+    for i in range(n):
+        if i == 8:
+            wf.evaluator.temperature = 4.0
+            wf.forwards[1].eps = 0.01
+        st.step()
+        if i % 3 == 0:             # eager work between the replays
+            torch.cuda.synchronize()
+            torch.ones(100, device="cuda").sum().item()
+    torch.cuda.synchronize()
+    return wf, st
+
+
+def test_a_captured_step_follows_the_temperature(tmp_path):
+    ends = []
+    for graph in (False, True):
+        wf, st = steps(tmp_path, graph)
+        if graph:
+            assert st._graph is not None, getattr(st, "capture_error", "")
+        ends.append([f.weights.devmem.clone() for f in wf.forwards] +
+                    [wf.evaluator.loss.devmem.clone(),
+                     wf.evaluator.n_err.devmem.clone(),
+                     wf.forwards[-1].max_idx.devmem.clone()])
+    for a, b in zip(*ends):
+        assert torch.equal(a, b)

@@ -25,9 +25,10 @@ Replayability invariants (the units were built for these):
   ``last_minibatch``, which runs after the replay);
 * dropout's PRNG step counter lives in device memory and is advanced by
   a leading bump kernel (dropout.py), so each replay draws fresh masks;
-* hyper-parameters passed by value into kernels (learning rate, decay)
-  are part of :meth:`_signature`; a change drops the graph and the next
-  train step re-captures.
+* hyper-parameters passed by value into kernels (learning rate, decay,
+  a distillation's temperature, a layer norm's eps) are part of
+  :meth:`_signature`; a change drops the graph and the next train step
+  re-captures.
 
 The stepper only replays full-size TRAIN minibatches; short or
 valid/test minibatches take the eager path (which also honours
@@ -140,6 +141,9 @@ class GraphStepper(object):
                         float(getattr(g, "learning_rate_bias", 0.0)),
                         float(getattr(g, "weights_decay", 0.0)),
                         float(getattr(g, "gradient_moment", 0.0))))
+        sig.append(float(getattr(self.evaluator, "temperature", 0.0)))
+        sig.append(tuple(float(getattr(f, "eps", 0.0))
+                         for f in self.forwards))
         return tuple(sig)
 
     def _capture(self):
