@@ -24,6 +24,19 @@ def student(tmp_path, device, **kw):
                  **kw)
 
 
+def test_likeliest_class_of_a_distilled_head(tmp_path):
+    """Who links max_idx has the class of the largest logit."""
+    wf = student(tmp_path, NumpyDevice())
+    head = wf.forwards[-1]
+    for _ in range(2):
+        wf.loader.run()
+        for f in wf.forwards:
+            f.run()
+        numpy.testing.assert_array_equal(head.max_idx.mem,
+                                         head.output.mem.argmax(axis=1))
+        assert len(set(head.max_idx.mem.tolist())) > 1
+
+
 def stepper(wf):
     from veles.znicz_amd.hipgraph import GraphStepper
     wf.comm_sync = None            # (what run() would have; not used here)

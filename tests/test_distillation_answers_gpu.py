@@ -49,3 +49,30 @@ def test_a_captured_step_follows_the_temperature(tmp_path):
                      wf.forwards[-1].max_idx.devmem.clone()])
     for a, b in zip(*ends):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_likeliest_class_of_a_distilled_head(tmp_path, graph):
+    wf, _ = steps(tmp_path, graph, 6)
+    head = wf.forwards[-1]
+    want = head.output.devmem.argmax(1)
+    assert len(set(want.tolist())) > 1
+    head.max_idx.map_read()
+    assert head.max_idx.mem.tolist() == want.tolist()
+
+
+def test_likeliest_class_of_rows_that_have_none(tmp_path):
+    """It stays a class where there is no largest logit."""
+    dev = ROCmDevice(0)
+    wf = student(tmp_path, dev, n_valid=0)
+    wf.loader.run()
+    head = wf.forwards[-1]
+    for f in wf.forwards[:-1]:
+        f.run()
+    head.input.devmem[3].fill_(float("nan"))
+    head.input.touch_device()
+    head.run()
+    idx = head.max_idx.devmem.tolist()
+    want = head.output.devmem.argmax(1).tolist()
+    assert 0 <= idx[3] < 10
+    assert idx[:3] + idx[4:] == want[:3] + want[4:]

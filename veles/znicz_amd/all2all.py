@@ -126,8 +126,10 @@ class All2AllSoftmax(All2All):
     MAPPING = "softmax"
     ACTIVATION = act.ACT_LINEAR
 
-    #: leave the logits in ``output`` (no softmax, no ``max_idx``): set by
-    #: who asks for log probabilities instead of probabilities
+    #: leave the logits in ``output`` (no softmax): set by who asks for log
+    #: probabilities instead of probabilities.  ``max_idx`` is that of the
+    #: logits; in ``forward_mode`` (a teacher, a served model's top answers)
+    #: it is not written, since the answers are the classes themselves
     logits_only = False
 
     def __init__(self, workflow, **kwargs):
@@ -148,11 +150,13 @@ class All2AllSoftmax(All2All):
 
     def numpy_run(self):
         super(All2AllSoftmax, self).numpy_run()
-        if self.logits_only:
+        if self.logits_only and self.forward_mode:
             return
         v = self.output.mem
         self.max_idx.map_invalidate()
         self.max_idx.mem[...] = numpy.argmax(v, axis=1)
+        if self.logits_only:
+            return
         m = v.max(axis=1, keepdims=True)
         e = numpy.exp(v - m)
         self.output.mem[...] = e / e.sum(axis=1, keepdims=True)
@@ -164,6 +168,20 @@ class All2AllSoftmax(All2All):
                     bias=self.bias.devmem if self.include_bias else None)
         self.output.touch_device()
         if self.logits_only:
+            if not self.forward_mode:
+                self._hip_max_idx()
             return
         ops.softmax_fwd(self.output.devmem, self.max_idx.devmem)
+        self.max_idx.touch_device()
+
+    def _hip_max_idx(self):
+        """``max_idx`` of rows of logits; a row that has no likeliest class
+        (NaN or plus infinity in it) is of class 0."""
+        import torch
+        from veles.znicz_amd import ops
+        idx = self.max_idx.devmem
+        ops.token_logprobs(
+            self.output.devmem, top_idx=idx.view(-1, 1),
+            top_logprob=torch.empty(idx.shape[0], 1, device=idx.device))
+        idx.clamp_(min=0)
         self.max_idx.touch_device()
