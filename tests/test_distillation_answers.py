@@ -55,3 +55,19 @@ def test_signature_of_a_captured_step(tmp_path, change):
     else:
         wf.forwards[1].eps = 1e-3
     assert st._signature() != before
+
+
+def test_statistics_are_not_written_in_forward_mode():
+    rng = numpy.random.RandomState(3)
+    fwd = LayerNormForward(DummyWorkflow())
+    fwd.input = Array(rng.normal(0, 1.5, (6, 12)).astype(numpy.float32))
+    assert fwd.initialize(device=NumpyDevice()) is not False
+    fwd.run()
+    y, mean = fwd.output.mem.copy(), fwd.mean.mem.copy()
+    assert mean.any() and fwd.rstd.mem.all()
+    fwd.forward_mode = True
+    fwd.mean.mem[...] = 7
+    fwd.rstd.mem[...] = 8
+    fwd.run()
+    assert (fwd.mean.mem == 7).all() and (fwd.rstd.mem == 8).all()
+    numpy.testing.assert_array_equal(fwd.output.mem, y)

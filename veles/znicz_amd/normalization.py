@@ -185,8 +185,7 @@ class LayerNormForward(Forward):
 
     def numpy_run(self):
         self.input.map_read()
-        for arr in (self.output, self.mean, self.rstd):
-            arr.map_invalidate()
+        self.output.map_invalidate()
         x = self.input.mem.reshape(-1, self.input.shape[-1])
         mean = x.mean(axis=1, keepdims=True)
         xc = x - mean
@@ -195,8 +194,11 @@ class LayerNormForward(Forward):
         y = xc * rstd * self.weights.mem
         if self.include_bias:
             y = y + self.bias.mem
-        self.mean.mem[...] = mean[:, 0]
-        self.rstd.mem[...] = rstd[:, 0]
+        if not self.forward_mode:
+            self.mean.map_invalidate()
+            self.rstd.map_invalidate()
+            self.mean.mem[...] = mean[:, 0]
+            self.rstd.mem[...] = rstd[:, 0]
         self.output.mem[...] = y.reshape(self.output.shape)
 
     def hip_run(self):
