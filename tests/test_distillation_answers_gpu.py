@@ -76,3 +76,24 @@ def test_likeliest_class_of_rows_that_have_none(tmp_path):
     want = head.output.devmem.argmax(1).tolist()
     assert 0 <= idx[3] < 10
     assert idx[:3] + idx[4:] == want[:3] + want[4:]
+
+
+def test_graphs_of_top_answers_are_few(tmp_path):
+    from veles.serving import InferenceEngine
+    eng = InferenceEngine(teacher_file(tmp_path), device=ROCmDevice(0))
+    rng = numpy.random.RandomState(2)
+    x = rng.normal(0, 1, (45, 24)).astype(numpy.float32)
+    labels = rng.randint(-1, 10, 45)
+    most = eng.predict_top(x, 128, labels)
+    assert most["top"].shape == most["top_logprob"].shape == (45, 128)
+    for top in list(range(1, 129, 3)) + [8, 9, 16, 128, 5]:
+        ans = eng.predict_top(x, top, labels)
+        assert ans["top"].shape == (45, top)
+        numpy.testing.assert_array_equal(ans["top"], most["top"][:, :top])
+        numpy.testing.assert_array_equal(ans["top_logprob"],
+                                         most["top_logprob"][:, :top])
+        for k in ("logprob", "entropy"):
+            numpy.testing.assert_array_equal(ans[k], most[k])
+    graphs = {id(v[0]) for v in eng._top_graphs.values()}
+    assert len(graphs) <= 5
+    assert all(v[0] is not None for v in eng._top_graphs.values())

@@ -28,6 +28,10 @@ import numpy
 class InferenceEngine(object):
     """Snapshot → forward-only executor with fixed-batch graph replay."""
 
+    #: alternatives of the passes that predict_top captures: requests of any
+    #: other number take the first ones of the next larger list
+    TOP_SIZES = (8, 16, 32, 64, 128)
+
     def __init__(self, snapshot_path, device=None, batch_size=None):
         from veles.snapshotter import SnapshotterBase
         wf = SnapshotterBase.import_(snapshot_path)
@@ -51,7 +55,9 @@ class InferenceEngine(object):
         self.batch_size = batch_size or int(wf.loader.max_minibatch_size)
         self._in = wf.loader.minibatch_data
         self._graph = None
-        self._top_graphs = {}          # alternatives -> (graph, outputs)
+        #: alternatives -> (graph, run, outputs), which all that have the
+        #: same of TOP_SIZES share
+        self._top_graphs = {}
         self._lock = threading.Lock()
 
     # -- core ---------------------------------------------------------------
@@ -159,16 +165,17 @@ class InferenceEngine(object):
         from veles.znicz_amd import ops
         self._upload(x)
         out = self.forwards[-1].output
-        if top not in self._top_graphs:
+        size = min(s for s in self.TOP_SIZES if s >= top)
+        if size not in self._top_graphs:
             batch, dev = out.devmem.shape[0], out.devmem.device
             outs = {
                 "labels": torch.full((batch,), -1, dtype=torch.int32,
                                      device=dev),
                 "logprob": torch.empty(batch, device=dev),
                 "entropy": torch.empty(batch, device=dev),
-                "top": torch.empty(batch, top, dtype=torch.int32,
+                "top": torch.empty(batch, size, dtype=torch.int32,
                                    device=dev),
-                "top_logprob": torch.empty(batch, top, device=dev)}
+                "top_logprob": torch.empty(batch, size, device=dev)}
 
             def run():
                 self._forward_logits()
@@ -185,8 +192,9 @@ class InferenceEngine(object):
                 graph = g
             except Exception:          # eager, permanently
                 graph = None
-            self._top_graphs[top] = (graph, run, outs)
-        graph, run, outs = self._top_graphs[top]
+            self._top_graphs[size] = (graph, run, outs)
+        graph, run, outs = self._top_graphs.setdefault(
+            top, self._top_graphs[size])
         given = numpy.full(outs["labels"].shape[0], -1, numpy.int32)
         if labels is not None:
             given[:len(labels)] = labels
@@ -197,8 +205,11 @@ class InferenceEngine(object):
             run()
         out.touch_device()
         n = x.shape[0]
-        return {k: v[:n].cpu().numpy() for k, v in outs.items()
-                if k != "labels"}
+        ans = {k: v[:n].cpu().numpy() for k, v in outs.items()
+               if k != "labels"}
+        for k in ("top", "top_logprob"):
+            ans[k] = ans[k][:, :top]   # (a list in order)
+        return ans
 
     def _top_numpy(self, x, labels, top):
         from veles.znicz_amd.distillation import numpy_logprobs
