@@ -97,3 +97,35 @@ def test_graphs_of_top_answers_are_few(tmp_path):
     graphs = {id(v[0]) for v in eng._top_graphs.values()}
     assert len(graphs) <= 5
     assert all(v[0] is not None for v in eng._top_graphs.values())
+
+
+@pytest.mark.parametrize("head", ["softmax", "all2all"])
+def test_predict_copies_an_answer_once(tmp_path, head):
+    """Out of the pinned buffer, which the next batch overwrites; a bf16
+    head's numbers are copied by their conversion."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from veles.serving import InferenceEngine
+
+    class Copies(TorchDispatchMode):
+        n = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if func in (torch.ops.aten._to_copy.default,
+                        torch.ops.aten.clone.default):
+                Copies.n += 1
+            return func(*args, **(kwargs or {}))
+
+    path = teacher_file(tmp_path)
+    wf = build(mlp(head=head), ROCmDevice(0), loss="distillation",
+               distill={"snapshot": path, "top": 4})
+    eng = InferenceEngine(save(wf, tmp_path, "copied"),
+                          device=ROCmDevice(0))
+    x = numpy.random.RandomState(2).normal(0, 1, (20, 24))
+    eng.predict(x)
+    Copies.n = 0
+    with Copies():
+        a = eng.predict(x)
+    assert Copies.n == 1
+    b = a.copy()
+    eng.predict(x * 2)
+    numpy.testing.assert_array_equal(a, b)

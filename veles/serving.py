@@ -125,9 +125,9 @@ class InferenceEngine(object):
                                         dtype=out.devmem.dtype,
                                         pin_memory=True)
         self._out_pin.copy_(out.devmem)
-        # (a copy: .float() of an fp32 head is the pinned buffer itself,
-        # which the next batch overwrites)
-        return self._out_pin[:n].float().clone().numpy()
+        # (a copy of any head's numbers, once: those of an fp32 one would
+        # else lie in the pinned buffer, which the next batch overwrites)
+        return self._out_pin[:n].to(torch.float32, copy=True).numpy()
 
     def _run_numpy(self, x):
         self._in.map_invalidate()
