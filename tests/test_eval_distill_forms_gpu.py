@@ -1,0 +1,51 @@
+"""eval_distill on the GPU in the form in which the evaluator calls it (fp32
+logits, a bf16 gradient, labels and n_err), its count of errors beside what
+is wrong with the teacher, and classes that are named more than once."""
+
+import math
+
+import numpy
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("no GPU", allow_module_level=True)
+
+from test_row_ops_gpu import (  # noqa: E402
+    E32, INF, TYPES, check_distill, cuda, f64, logits_case, rows_of,
+    teacher_case)
+from veles.znicz_amd import ops  # noqa: E402
+
+
+def counted(tx, idx, z, err, labels, batch=None, tau=1.0):
+    """(loss, n_err) of a call that counts from 10 on"""
+    loss = torch.full((tx.shape[0],), 55.0, device="cuda")
+    n = torch.tensor([10, 3], dtype=torch.int32).cuda()
+    ops.eval_distill(tx, cuda(idx), cuda(z), err, loss, batch, tau,
+                     torch.as_tensor(labels, dtype=torch.int32).cuda(), n)
+    assert n[1].item() == 3
+    return loss, n[0].item() - 10
+
+
+@pytest.mark.parametrize("R", [6, 66])
+@pytest.mark.parametrize("C", [12, 1000, 50001])
+@pytest.mark.parametrize("name", sorted(TYPES))
+def test_errors_are_the_students_alone(R, C, name):
+    """A teacher's class that does not exist, or a logit of it that is no
+    number, leaves the student's likeliest class what it is."""
+    tx = rows_of(logits_case(R, C, 2), TYPES[name])
+    idx, z = teacher_case(R, C, 4)
+    z[0::6, 1] = numpy.nan
+    z[1::6, 3] = INF
+    idx[2::6, 0] = C
+    idx[3::6, 2] = 2 ** 31 - 1
+    z[4::6] = -INF
+    labels = f64(tx).argmax(1)
+    loss, n = counted(tx, idx, z, torch.empty_like(tx), labels)
+    assert n == 0
+    bad = numpy.isin(numpy.arange(R) % 6, (0, 1, 2, 3))
+    assert (numpy.isnan(f64(loss)) == bad).all()
+    labels[::2] = (labels[::2] + 1) % C
+    assert counted(tx, idx, z, torch.empty_like(tx), labels)[1] == R // 2

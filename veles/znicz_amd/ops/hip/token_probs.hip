@@ -1147,8 +1147,9 @@ __global__ __launch_bounds__(THREADS) void distill_k(DistillArgs a) {
     if (tid == 0) {
       if (a.loss) a.loss[at.row] = loss;
       if (a.labels) {
+        // (the student's errors: what the teacher gives is no part of them)
         const int l = a.labels[at.row];
-        if (l >= 0 && (bad || r.none || first != l)) atomicAdd(a.n_err, 1);
+        if (l >= 0 && (r.bad || r.none || first != l)) atomicAdd(a.n_err, 1);
       }
     }
   }
