@@ -29,6 +29,41 @@ def counted(tx, idx, z, err, labels, batch=None, tau=1.0):
     return loss, n[0].item() - 10
 
 
+# (up to 16384 classes of fp32 a row of 256 threads, to 32768 one of 512, to
+# 65536 one of 1024, longer ones read twice; 64 rows or fewer may be cut)
+@pytest.mark.parametrize("R", [9, 65, 97])
+@pytest.mark.parametrize("C", [10, 1000, 5003, 16384, 20001, 50001, 140007])
+@pytest.mark.parametrize("xpad,epad", [(0, 0), (1, 3)])
+def test_form_of_the_evaluator(R, C, xpad, epad):
+    rng = numpy.random.RandomState(C)
+    x = logits_case(9, C, C)[numpy.arange(R) % 9]
+    x[R // 2] = -INF
+    x[R // 3, C // 2] = numpy.nan
+    x[3, C - 2:] = 30.0                       # the first of two
+    x[5] = -2.0 ** 15                         # far below 0, as one
+    tx = rows_of(x, torch.float32, xpad)
+    k = min(C, 16)
+    idx, z = teacher_case(R, C, k, 5)
+    idx[1] = -1
+    z[2, k // 2:] = -INF
+    err = rows_of(numpy.full((R, C), 55.0), torch.bfloat16, epad)
+    xs = f64(tx)
+    none = numpy.isnan(xs).any(1) | (xs == -INF).all(1)
+    labels = numpy.where(none, 0, xs.argmax(1))
+    labels[::4] = rng.randint(0, C, len(labels[::4]))
+    labels[7] = -1
+    live = R - 1
+    loss, n = counted(tx, idx, z, err, labels, live, 2.0)
+    check_distill(tx, xs, idx, z, 2.0, err, loss, live)
+    wrong = none | (xs.argmax(1) != labels)
+    assert n == (wrong & (labels >= 0))[:live].sum()
+    if epad:
+        buf = err.as_strided((R * (C + epad),), (1,), 0)
+        keep = torch.ones_like(buf, dtype=torch.bool)
+        keep.as_strided((R, C), (C + epad, 1), 0).fill_(False)
+        assert torch.isnan(buf[keep]).all()
+
+
 @pytest.mark.parametrize("R", [6, 66])
 @pytest.mark.parametrize("C", [12, 1000, 50001])
 @pytest.mark.parametrize("name", sorted(TYPES))
