@@ -71,3 +71,26 @@ def test_statistics_are_not_written_in_forward_mode():
     fwd.run()
     assert (fwd.mean.mem == 7).all() and (fwd.rstd.mem == 8).all()
     numpy.testing.assert_array_equal(fwd.output.mem, y)
+
+
+@pytest.mark.parametrize("tau", [1.0, 2.5])
+def test_loss_of_a_class_that_is_named_twice(tau):
+    """It has both shares, in the loss as in the gradient: as if it were
+    named once, with the logit that has their sum."""
+    rng = numpy.random.RandomState(1)
+    x = rng.normal(0, 2, (3, 30))
+    idx = numpy.array([[4, 7, 4, 9], [5, 5, 5, 5], [1, 2, 2, 1]])
+    z = rng.normal(0, 2, (3, 4))
+    loss, grad = numpy_distill(x, idx, z, tau)
+    for i in range(3):
+        at = sorted(set(idx[i].tolist()))
+        one = [tau * numpy.logaddexp.reduce(z[i][idx[i] == a] / tau)
+               for a in at]
+        want_l, want_g = numpy_distill(x[i:i + 1], [at], [one], tau)
+        # a few roundings of 64 bits, of numbers below 20
+        assert abs(loss[i] - want_l[0]) < 1e-12
+        numpy.testing.assert_allclose(grad[i], want_g[0], atol=1e-13)
+    # (one sure class, of which the student is as sure)
+    x = numpy.full((1, 4), -50.0)
+    x[0, 2] = 0.0
+    assert abs(numpy_distill(x, [[2, 2]], [[0.0, 0.0]], tau)[0][0]) < 1e-6

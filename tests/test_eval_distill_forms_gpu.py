@@ -84,3 +84,50 @@ def test_errors_are_the_students_alone(R, C, name):
     assert (numpy.isnan(f64(loss)) == bad).all()
     labels[::2] = (labels[::2] + 1) % C
     assert counted(tx, idx, z, torch.empty_like(tx), labels)[1] == R // 2
+
+
+@pytest.mark.parametrize("R", [5, 70])
+@pytest.mark.parametrize("C", [40, 1000, 50001, 140007])
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("tau", [0.7, 4.0])
+def test_a_class_that_is_named_twice(R, C, name, tau):
+    """Loss and gradient are those of the class named once, with the logit
+    that has the sum of its shares."""
+    rng = numpy.random.RandomState(C + R)
+    tx = rows_of(logits_case(R, C, 6), TYPES[name])
+    at, once = teacher_case(R, C, 6, 3)
+    once -= numpy.float32(500.0)              # (a shift has no effect)
+    # each of them again and again, 128 places in all, out of order
+    part = rng.normal(0, 2, (R, 6, 21))
+    part -= numpy.logaddexp.reduce(part / tau, axis=2)[:, :, None] * tau
+    idx = numpy.repeat(at[:, :, None], 21, 2).reshape(R, 126)
+    z = (once[:, :, None] + part).reshape(R, 126)
+    order = rng.permutation(126)
+    idx, z = idx[:, order], z[:, order].astype(numpy.float32, "C")
+    idx = numpy.ascontiguousarray(idx)
+    err = torch.empty_like(tx)
+    loss, _ = counted(tx, idx, z, err, numpy.zeros(R, int), tau=tau)
+    joined = numpy.zeros((R, 6))
+    for i in range(R):
+        for j in range(6):
+            same = idx[i] == at[i, j]
+            joined[i, j] = tau * numpy.logaddexp.reduce(
+                z[i, same].astype(float) / tau)
+    check_distill(tx, f64(tx), at, joined, tau, err, loss)
+
+
+@pytest.mark.parametrize("C", [50, 50001])
+@pytest.mark.parametrize("R", [3, 80])
+def test_a_divergence_is_not_below_zero(R, C):
+    """A student that is as sure as a teacher whose only class is named four
+    times."""
+    x = numpy.full((R, C), -60.0)
+    x[:, C // 2] = 0.0
+    tx = rows_of(x, torch.float32)
+    idx = numpy.full((R, 4), C // 2, numpy.int32)
+    z = numpy.tile(numpy.float32([0.0, 1.0, -3.0, 2.0]), (R, 1))
+    loss, _ = counted(tx, idx, z, torch.empty_like(tx),
+                      numpy.full(R, C // 2))
+    # four shares and their four logarithms, a few steps of fp32 each
+    assert (numpy.abs(f64(loss)) <= 4 * 16 * E32).all()
+    assert not any(math.isnan(v) for v in f64(loss))

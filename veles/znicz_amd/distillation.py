@@ -82,12 +82,16 @@ def numpy_distill(logits, top_idx, top_logit, temperature):
         lnp -= numpy.log(numpy.exp(lnp).sum())
         lnq = (zi - zi.max()) / tau
         lnq -= numpy.log(numpy.exp(lnq).sum())
-        q = numpy.exp(lnq)
+        # (all places of a class together)
+        at, place = numpy.unique(at, return_inverse=True)
+        joined = numpy.full(len(at), -numpy.inf)
+        numpy.logaddexp.at(joined, place, lnq)
+        q = numpy.exp(joined)
         some = q > 0
-        loss[i] = tau * tau * (q[some] * (lnq[some] -
+        loss[i] = tau * tau * (q[some] * (joined[some] -
                                           lnp[at[some]])).sum()
         grad[i] = numpy.exp(lnp)
-        numpy.subtract.at(grad[i], at, q)
+        grad[i, at] -= q
         grad[i] *= tau
     return loss, grad
 

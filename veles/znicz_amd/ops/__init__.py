@@ -339,12 +339,14 @@ def eval_distill(logits, top_idx, top_logit, err_out, loss=None, batch=None,
     ``err_out`` has the logits' type and shape and may be ``logits`` itself;
     that of fp32 logits may be bf16.  Other outputs lie apart from all else.
     Places with a negative class or a logit of minus infinity are empty; a
-    class that is named twice has both shares.  A row without a named class,
-    or whose logits are all minus infinity, has no loss and no gradient; one
-    with NaN, plus infinity or a class of V or more gives NaN.  Rows from
-    ``batch`` on are padding and hold zeros.  With ``labels`` int32[rows],
-    ``n_err[0]`` (int32) grows by the rows whose likeliest class is another
-    (labels below 0 are none)."""
+    class that is named twice has the sum of both shares as its q, in the
+    loss as in the gradient.  A row without a named class, or whose logits
+    are all minus infinity, has no loss and no gradient; one with NaN, plus
+    infinity or a class of V or more gives NaN.  Rows from ``batch`` on are
+    padding and hold zeros.  With ``labels`` int32[rows], ``n_err[0]``
+    (int32) grows by the rows whose likeliest class is another by the
+    student's logits, whatever the teacher gives (labels below 0 are none).
+    """
     x = _rows(logits)
     require().eval_distill(x, top_idx, top_logit, _rows(err_out), loss,
                            x.shape[0] if batch is None else int(batch),

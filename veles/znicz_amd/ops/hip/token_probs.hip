@@ -853,8 +853,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_k(
 // ---------------------------------------------------------------------------
 // eval_distill
 // ---------------------------------------------------------------------------
-// q = softmax(z / tau) over the teacher's classes, p = softmax(x / tau) over
-// all;  loss = tau^2 sum q (ln q - ln p),  dloss/dx_j = tau (p_j - q_j).
+// q = softmax(z / tau) over the teacher's classes (one that is named more than
+// once has the sum of its shares), p = softmax(x / tau) over all;  loss = tau^2 sum q (ln q - ln p),  dloss/dx_j = tau (p_j - q_j).
 // The row is read once: it stays in registers until its sum is known.  The
 // teacher's classes are taken off the gradients in registers too, by the
 // threads that hold them, so that each gradient is written once.
@@ -898,7 +898,7 @@ struct DistillSpace {
 // and i + 64.
 struct Teacher {
   int id[2];
-  float z[2], x[2], q[2];
+  float z[2], x[2], q[2];      // (z: from softmax on less the largest, zm)
   float zm, gs;
   bool wrong;
 
@@ -940,14 +940,19 @@ struct Teacher {
     zm = wave_max(fmaxf(z[0], z[1]));
     float g[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      g[h] = id[h] >= 0 ? pow2((z[h] - zm) * a.c) : 0.f;
+    for (int h = 0; h < 2; ++h) {
+      z[h] -= zm;
+      g[h] = id[h] >= 0 ? pow2(z[h] * a.c) : 0.f;
+    }
     gs = wave_sum(g[0] + g[1]);
 #pragma unroll
     for (int h = 0; h < 2; ++h) q[h] = g[h] / gs;
   }
   // Leaves what each class takes off its gradient, all places of a class
-  // together, with the thread that holds the element of x[0..n).
+  // together, with the thread that holds the element of x[0..n).  Places that
+  // share a class get the logit z that belongs to the sum Q of their shares
+  // (tau ln Q/q more), so that the loss, which goes over the places, is
+  // sum Q (ln Q - ln p) over the classes.
   template <typename T, int THREADS, int NV>
   __device__ __forceinline__ void place(const DistillArgs& a, int base, int n,
                                         const Cut<T>& cut,
@@ -979,6 +984,8 @@ struct Teacher {
     for (int h = 0; h < 2; ++h) {
       const int k = tid + h * WAVE;
       const int j = id[h] - base;
+      if (q[h] > 0.f && sum[h] != q[h])
+        z[h] = fmaf(a.tau * LN2, log2_of(sum[h] / q[h]), z[h]);
       sp.id[k] = -1;
       if (again[h] || j < 0 || j >= n) continue;
       sp.id[k] = j;
@@ -998,14 +1005,14 @@ struct Teacher {
       atomicOr(&sp.where[owner], 1u << bit);
     }
   }
-  // tau sum q (ln q - ln p)
+  // tau sum q (ln q - ln p), after place()
   __device__ __forceinline__ float loss(const DistillArgs& a, const Row& r) {
     const float apart = a.tau * (r.ln - log2_of(gs) * LN2);
     float s = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       if (id[h] >= 0 && q[h] > 0.f)
-        s += q[h] * ((z[h] - zm) - (x[h] - r.m) + apart);
+        s += q[h] * (z[h] - (x[h] - r.m) + apart);
     return wave_sum(s);
   }
 };
