@@ -66,6 +66,14 @@ __device__ __forceinline__ int wave_sum(int v) {
   return wave_join(v, [](int a, int b) { return a + b; });
 }
 
+// What the lanes of a wave have written to LDS, or read from it, before this is
+// done for those that read, or write, it afterwards.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Sum over the workgroup, in every thread.  `tmp`: one float for each wave,
 // free again after the call.
 __device__ __forceinline__ float block_sum(float v, float* tmp) {

@@ -964,7 +964,7 @@ struct Teacher {
       sp.id[tid + h * WAVE] = id[h];
       sp.take[tid + h * WAVE] = q[h];
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_fence();
     float sum[2] = {0.f, 0.f};
     bool again[2] = {id[0] < 0, id[1] < 0};
 #pragma unroll 4
@@ -978,8 +978,8 @@ struct Teacher {
         again[h] |= same && j < tid + h * WAVE;
       }
     }
-    // (one wave: all its reads are before its writes)
-    __builtin_amdgcn_wave_barrier();
+    // (all reads of the wave are before its writes)
+    wave_fence();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = tid + h * WAVE;
