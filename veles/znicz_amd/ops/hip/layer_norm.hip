@@ -221,8 +221,8 @@ __global__ __launch_bounds__(LN_THREADS) void ln_join_k(
 // ---------------------------------------------------------------------------
 // rows in registers
 // ---------------------------------------------------------------------------
-// A team of lanes has a row, 8 or 16 elements a lane: a part of a wave, a
-// wave, or a whole workgroup, as the row is long.  It goes through the rows
+// A team of lanes has a row, 8, 16 or (forward) 32 elements a lane: a part of a
+// wave, a wave, or a whole workgroup, as the row is long.  It goes through the rows
 // in steps, several at a time, with the gain and the shift (backward: the
 // gain and the two column sums) in registers all along.
 

@@ -88,18 +88,6 @@ __device__ __forceinline__ float block_sum(float v, float* tmp) {
   return v;
 }
 
-__device__ __forceinline__ float block_max(float v, float* tmp) {
-  const int waves = blockDim.x / WAVE;
-  v = wave_max(v);
-  if (waves == 1) return v;
-  if ((threadIdx.x & (WAVE - 1)) == 0) tmp[threadIdx.x / WAVE] = v;
-  __syncthreads();
-  v = tmp[0];
-  for (int i = 1; i < waves; ++i) v = fmaxf(v, tmp[i]);
-  __syncthreads();
-  return v;
-}
-
 // The largest of three, NaN left aside.  (fmaxf of loaded values takes two
 // more instructions each, which make them canonical.)
 __device__ __forceinline__ float max3(float a, float b, float c) {
