@@ -5,7 +5,7 @@ test_distillation_answers_gpu.py)."""
 import numpy
 import pytest
 
-from test_distillation import build, mlp, teacher_file
+from test_distillation import build, mlp, save, teacher_file
 from veles import prng
 from veles.backends import NumpyDevice
 from veles.dummy import DummyWorkflow
@@ -94,3 +94,32 @@ def test_loss_of_a_class_that_is_named_twice(tau):
     x = numpy.full((1, 4), -50.0)
     x[0, 2] = 0.0
     assert abs(numpy_distill(x, [[2, 2]], [[0.0, 0.0]], tau)[0][0]) < 1e-6
+
+
+def test_a_softmax_within_the_teacher_stays_one(tmp_path):
+    """Its last layer alone gives logits."""
+    for key in ("default", "loader"):
+        prng.get(key)
+    prng.seed_all(5)
+    wf = build([{"type": "softmax", "->": {"output_sample_shape": 12},
+                 "<-": {}},
+                {"type": "softmax", "->": {"output_sample_shape": 10},
+                 "<-": {}}], NumpyDevice())
+    wf.run()
+    path = save(wf, tmp_path, "within")
+    wf = build(mlp(), NumpyDevice(), loss="distillation",
+               distill={"snapshot": path, "top": 4})
+    wf.loader.run()
+    wf.teacher.run()
+    first, last = wf.teacher.forwards_
+    numpy.testing.assert_allclose(first.output.mem.sum(axis=1), 1.0,
+                                  rtol=1e-5)
+    assert not numpy.allclose(last.output.mem.sum(axis=1), 1.0)
+    # as the same model served: log probabilities in fp32 on both sides
+    from veles.serving import InferenceEngine
+    n = int(wf.loader.minibatch_size)
+    ans = InferenceEngine(path, device=NumpyDevice()).predict_top(
+        wf.loader.minibatch_data.mem[:n], 4)
+    numpy.testing.assert_array_equal(wf.teacher.top_idx.mem[:n], ans["top"])
+    numpy.testing.assert_array_equal(wf.teacher.top_logprob.mem[:n],
+                                     ans["top_logprob"])

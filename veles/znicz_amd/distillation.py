@@ -152,7 +152,7 @@ class TeacherAnswers(AcceleratedUnit):
         for f in self.forwards_:
             f.forward_mode = True
             if hasattr(f, "logits_only"):
-                f.logits_only = True
+                f.logits_only = f is self.forwards_[-1]
             f.initialize(device=device)
         batch = self.input.shape[0]
         out = self.forwards_[-1].output
