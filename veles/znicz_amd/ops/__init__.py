@@ -315,6 +315,10 @@ def token_logprobs(logits, labels=None, logprob=None, entropy=None,
       128: the likeliest classes, of equal ones the lower first.  Places
       without a class hold -1 and minus infinity.
 
+    Many equal values at the K-th place cost time (2048 rows of 131072 equal
+    bf16 logits, K = 64, 8.7 ms in place of 97 us): forbid classes with minus
+    infinity rather than with a type's lowest value.
+
     A logit of minus infinity forbids its class; a row of them has entropy 0
     and log probabilities of minus infinity.  A row with NaN or plus infinity
     gives NaN, and -1 for its classes.  Rows from ``batch`` on are padding:
@@ -405,7 +409,8 @@ def layer_norm_fwd(x, out, weights, bias, mean, rstd, eps=1e-5):
 
     x, out: bf16, fp16 or fp32, rows contiguous, any stride apart; ``out``
     may be ``x``.  weights, bias: fp32[C] or None; mean, rstd: fp32[rows],
-    written for the backward pass, or None, and apart from all else."""
+    written for the backward pass, or None, and apart from all else.  Sums
+    are in fp32: a row whose squared deviations pass its range has rstd 0."""
     require().layer_norm_fwd(_rows(x), _rows(out), weights, bias, mean,
                              rstd, float(eps))
 

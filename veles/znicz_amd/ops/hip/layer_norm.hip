@@ -295,7 +295,9 @@ __device__ __forceinline__ float mean_of(float sum, int cols, float per) {
 // the pack's before, too; a lane beyond the last pack has that one again.
 // Both are loaded and stored like any other (the same values to the same
 // place), which spares the branches, and are left out of the sums.  A row
-// shorter than a pack (TINY) is read and written one by one.
+// shorter than a pack (TINY) is read and written one by one.  Rows may begin at
+// any element; off multiples of 16 bytes loads and stores are slower: 16384 x
+// 4096 bf16, rows 4097 apart, 63 us instead of 50, backward 86 instead of 80.
 template <typename T, int TEAM, int NV, bool TINY>
 struct Slots {
   static constexpr int N = Pack<T>::N;

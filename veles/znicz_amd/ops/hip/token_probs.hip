@@ -472,7 +472,11 @@ __device__ __forceinline__ float share_bound(TopSpace<THREADS>& sp, int top) {
 
 // Too many classes reach the bound (one value many times): the top-th value
 // itself, then among the classes that hold it the last that is needed, by
-// halving; the part x[0..n) is read from the caches each time.
+// halving; the part x[0..n) is read from the caches each time, up to 32 + log2
+// n times with two barriers each.  Rows of one value, or with fewer classes than
+// alternatives above a finite lowest value, all come here: 256 x 1000 fp32 24
+// to 29 us in place of 4.5, 8192 x 8000 bf16 1.4 to 1.5 ms in place of 38 us,
+// 2048 x 131072 8.7 to 9.2 ms in place of 97 us.
 template <typename T, int THREADS>
 __device__ __forceinline__ void thin_out(const T* x, int n, int base, int top,
                                       TopSpace<THREADS>& sp) {
@@ -854,7 +858,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_k(
 // eval_distill
 // ---------------------------------------------------------------------------
 // q = softmax(z / tau) over the teacher's classes (one that is named more than
-// once has the sum of its shares), p = softmax(x / tau) over all;  loss = tau^2 sum q (ln q - ln p),  dloss/dx_j = tau (p_j - q_j).
+// once has the sum of its shares), p = softmax(x / tau) over all;
+//   loss = tau^2 sum q (ln q - ln p),  dloss/dx_j = tau (p_j - q_j).
 // The row is read once: it stays in registers until its sum is known.  The
 // teacher's classes are taken off the gradients in registers too, by the
 // threads that hold them, so that each gradient is written once.
@@ -879,7 +884,9 @@ struct DistillArgs {
 // Gradients of so many bytes are not in the caches any more when the next
 // operator reads them.  Stored past them: 2048 x 30000 bf16 (123 MB) 54
 // instead of 62 us, 2048 x 131072 220 instead of 224; but a kernel that reads
-// 67 MB just written takes 10 us longer (134 MB: 11 us less).
+// 67 MB just written takes 10 us longer (134 MB: 11 us less).  For gradients of
+// the logits' type; a bf16 gradient of fp32 logits is 8 bytes a lane and pack,
+// and goes through the caches.
 #define PAST_CACHES (96l << 20)
 
 template <int THREADS>
@@ -1089,7 +1096,12 @@ __device__ __forceinline__ void put_gradients(O* to, const float* g,
 // us, 5.1 TB/s.  Bound by memory and by the turns that a row takes: a compute
 // unit has registers for one row of 256 KB, so that nothing is loaded while it
 // is stored (a copy laid out the same takes 192 us of the 219).  Loading the
-// next row into the registers that the gradients leave was no faster.
+// next row into the registers that the gradients leave was no faster.  The form
+// that the evaluator calls, fp32 logits with a bf16 gradient, labels and n_err:
+// 1023 x 50001 71 us, 4.3 TB/s; 256 x 1000 4.8 us; the first largest class and
+// its barrier are 0.3 to 2 us of that.  Wrong rows add to one number, each for
+// itself: 4096 x 1000 takes 15 us with all of them right, 21 with a third of
+// them wrong and 53 with all wrong (eval_softmax: 9 and 53).
 template <typename T, typename O, int THREADS, int NV, bool JOINED>
 __global__ __launch_bounds__(THREADS) void distill_k(DistillArgs a) {
   __shared__ DistillSpace<THREADS> sp;
